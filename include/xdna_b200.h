@@ -525,6 +525,98 @@ int xdna_subsample_conv2d(const uint16_t *x_dev, int B, int ci, int hin, int win
                           uint16_t *out_dev, void *stream);
 
 
+/* ------------------------------------- serving ops: paged cache, int8 norm, logits */
+/* What a server's own decoder needs between the int8 / bf16 products above: a key-value cache in
+ * pages shared by many streams, attention of one new token over it, the residual RMS norm that
+ * feeds xdna_gemm_i8, and the last step from logits to the next token.  Pointers are device
+ * pointers on the current device (for a cache: its device), work is asynchronous on `stream`,
+ * nothing is allocated or waited for in a call (all of them may be captured in a CUDA graph);
+ * 0, or -1 with xdna_last_error() set and nothing enqueued.
+ *
+ * A paged cache describes caller-owned K and V pools of n_layers layers: element c of the row of
+ * (layer, page, head, slot) lies at layer * stride_layer + page * stride_page + head *
+ * stride_head + slot * stride_slot + c, in elements, K and V alike (two strides of 0: the
+ * contiguous [layer][page][head][slot][c]).  kv_type 0: bf16; 1: int8 with one f32 scale per row,
+ * k_scale / v_scale [n_layers][n_pages][n_kv_heads][page_size] (value = whole number * scale).
+ * head_dim 64, 128 or 256; rows 16-byte aligned.  A block table (int32, [n_seqs][table_width],
+ * rows table_stride apart) names the page of each page_size positions of a stream; entries past
+ * a stream's length are never read.  The handle holds a workspace and a status word: calls on
+ * one handle run in one stream at a time.  max_seqs bounds the streams of one attention call. */
+typedef struct {
+    int kv_type, n_layers, n_pages, page_size, n_kv_heads, head_dim, max_seqs;
+    void *k, *v;
+    int64_t stride_layer, stride_page, stride_head, stride_slot;
+    float *k_scale, *v_scale;
+} XdnaPagedCacheConfig;
+typedef struct XdnaPagedCache XdnaPagedCache;
+XdnaPagedCache *xdna_paged_cache_create(XdnaDevice *dev, const XdnaPagedCacheConfig *cfg);
+/* frees the handle and its workspace (after its calls have finished), not the pools */
+void xdna_paged_cache_free(XdnaPagedCache *c);
+/* Append n_tokens tokens' keys and values, rotated on the way, and rotate their queries.  q (NULL:
+ * none) [n_tokens][n_q_heads][head_dim], k and v [n_tokens][n_kv_heads][head_dim], bf16 or
+ * (src_f32) f32, tokens *_stride elements apart.  Token t is position tok_pos[t] (negative: the
+ * token is skipped, its q_out row zeroed) of stream tok_seq[t] (NULL: stream t).  rope
+ * [rope_rows][rot_dim] f32 (NULL, rot_dim 0: no rotation) holds a position's rot_dim / 2 cosines,
+ * then its sines; component pairs (i, i + rot_dim / 2), or (2i, 2i + 1) when interleaved, are
+ * turned by angle i: (a cos - b sin, b cos + a sin), each product and sum rounded to f32; rot_dim a
+ * multiple of 16 up to head_dim, the other components pass.  q_out [n_tokens][n_q_heads][head_dim]
+ * bf16, disjoint from the inputs.  bf16 pools: rounded once; int8 pools, per row: scale =
+ * max|x| / 127 (1 for a zero row), whole number = x * (127 * (1 / max|x|)), each step rounded to
+ * f32, then half to even.  No two tokens
+ * of a call may be the same position of one stream. */
+int xdna_paged_append(XdnaPagedCache *c, int layer, int n_tokens, int n_q_heads, int src_f32, const void *q,
+                      int64_t q_stride, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                      const int32_t *tok_seq, const int32_t *tok_pos, const int32_t *block_table, int n_seqs,
+                      int table_width, int64_t table_stride, const float *rope, int rope_rows, int rot_dim,
+                      int interleaved, uint16_t *q_out, void *stream);
+/* Attention of one new token per stream: out [n_seqs][n_q_heads][head_dim] bf16 = softmax(scale
+ * q k^T) v over the stream's positions max(0, seq_lens - window) .. seq_lens - 1 (window 0: all);
+ * q bf16, streams q_stride elements apart; query head h reads K/V head h / (n_q_heads /
+ * n_kv_heads).  Scores, softmax and sums in f32, the weights to 16 bits of mantissa.  A stream
+ * of no positions (seq_lens <= 0) gives zeros.  lse (NULL: none) [n_seqs][n_q_heads] f32: the
+ * log of the sum of exponentials, -inf for no positions. */
+int xdna_paged_attention(XdnaPagedCache *c, int layer, const uint16_t *q, int64_t q_stride, int n_q_heads,
+                         const int32_t *block_table, int n_seqs, int table_width, int64_t table_stride,
+                         const int32_t *seq_lens, float scale, int window, uint16_t *out, float *lse, void *stream);
+/* Wait for `stream`, then report what the calls since the last check met in their device inputs:
+ * a page id outside the pool, a position past the table or the rope rows, a stream index out of
+ * range (such rows are skipped: not written, or left out of the softmax).  0, or -1. */
+int xdna_paged_cache_check(XdnaPagedCache *c, void *stream);
+
+/* Residual RMS norm with int8 rows: r = x + residual (NULL: x), y = r / sqrt(mean(r^2) + eps) * g
+ * with g = gamma (+ 1 when unit_offset), in f32 over the unrounded r.  x and residual are bf16 or
+ * (x_f32 / res_f32) f32, rows x_stride / res_stride elements apart; gamma f32 [D].  Outputs, each
+ * nullable but not all: residual_out [M][D] (type of residual; rows res_stride apart; may be
+ * residual itself), y_bf16 [M][D], and q8 [M][D] with scale [M] (both or none): scale = max|y| /
+ * 127 (1 for a zero row), q8 = r g * (127 * (1 / max|r g|)) half to even, the A operand of xdna_gemm_i8
+ * with rows_per_clip 1.  1 <= D <= 16384. */
+int xdna_rmsnorm_residual_i8(const void *x, int x_f32, int64_t x_stride, const void *residual, int res_f32,
+                             int64_t res_stride, const float *gamma, int unit_offset, float eps, int M, int D,
+                             void *residual_out, uint16_t *y_bf16, int8_t *q8, float *scale, void *stream);
+
+/* From logits to the next greedy token.  logits [B][V] bf16 or (src_f32) f32, rows logits_stride
+ * apart.  In this order, per row b and token id i, each step rounded to f32:
+ *   repetition [B]   x = x > 0 ? x / repetition[b] : x * repetition[b]   if i occurs in the history
+ *   frequency  [B]   x -= count * frequency[b]       count: occurrences among the generated tokens
+ *   presence   [B]   x -= presence[b]                if count > 0
+ *   bias             x += bias[j] for bias_ids[j] = i, j in [bias_start[b], bias_start[b + 1]);
+ *                    of several entries with one id the last counts
+ *   mask             x = -inf where bit i % 32 of mask[b * mask_stride + i / 32] is 0
+ * The history of row b is history[history_start[b] .. history_start[b + 1]), its first n_prompt[b]
+ * tokens (n_prompt NULL: none) are the prompt; ids outside [0, V) are passed over.  n_history and
+ * n_biases are the lengths of history and of bias: offsets are held within them.  Every one of the
+ * arrays may be NULL (history with history_start, the bias arrays together).  out [B][V] f32
+ * rows out_stride apart (may be logits itself if f32), ids [B] (NULL: none): the id of the
+ * largest result, the lowest of equals, NaN never, -1 when nothing is above -inf. */
+int xdna_logits_process(const void *logits, int src_f32, int64_t logits_stride, int B, int V,
+                        const int32_t *history, int n_history, const int32_t *history_start,
+                        const int32_t *n_prompt, const float *repetition, const float *frequency,
+                        const float *presence, const int32_t *bias_ids, const float *bias, int n_biases,
+                        const int32_t *bias_start,
+                        const uint32_t *mask, int64_t mask_stride, float *out, int64_t out_stride, int64_t *ids,
+                        void *stream);
+
+
 /* ------------------------------------------------- weight stores (npu-weights arena, npy dirs) */
 /* A baked weight arena: one safetensors file (rust/npu-weights/src/arena.rs:13-100) --
  * tensors BF16 or F32, "__metadata__" {format_version, arch, source_ref, source_fingerprint}.

@@ -798,3 +798,15 @@ class GemmaDecoder:
             self.close()
         except Exception:
             pass
+
+
+_SERVING = ("PagedCache", "process_logits", "rmsnorm_residual_i8", "rope_table")
+
+
+def __getattr__(name):
+    """The serving ops take torch tensors (serving.py); torch is imported with the first of them."""
+    if name in _SERVING:
+        from . import serving
+        globals().update({n: getattr(serving, n) for n in _SERVING})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

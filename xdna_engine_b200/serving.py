@@ -1,0 +1,292 @@
+"""The serving ops over torch tensors: a decoder's step between its int8 / bf16 products.
+
+PagedCache (append with rotary positions, attention of one new token), rmsnorm_residual_i8 and
+process_logits call the xdna_paged_*, xdna_rmsnorm_residual_i8 and xdna_logits_process entries of
+the C ABI on the tensors' memory.  All of them are asynchronous on `stream` (a raw cudaStream_t;
+None: torch's current stream of the tensors' device, so that torch's own ordering holds), and
+leave every tensor where it is: a tensor of the wrong type, shape, layout or device is refused with
+ValueError before anything is enqueued, and what the C ABI refuses raises XdnaError.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import XdnaError, _check, last_error, lib
+
+__all__ = ["PagedCache", "process_logits", "rmsnorm_residual_i8", "rope_table"]
+
+_FLOATS = (torch.bfloat16, torch.float32)
+
+
+class _PagedConfig(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("kv_type", "n_layers", "n_pages", "page_size", "n_kv_heads", "head_dim",
+                                       "max_seqs")] + \
+               [("k", C.c_void_p), ("v", C.c_void_p)] + \
+               [(n, C.c_int64) for n in ("stride_layer", "stride_page", "stride_head", "stride_slot")] + \
+               [("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+def _declare(L):
+    vp, i, i64, f = C.c_void_p, C.c_int, C.c_int64, C.c_float
+    L.xdna_paged_cache_create.argtypes = [vp, vp]
+    L.xdna_paged_cache_create.restype = vp
+    L.xdna_paged_cache_free.argtypes = [vp]
+    L.xdna_paged_append.argtypes = [vp, i, i, i, i, vp, i64, vp, i64, vp, i64, vp, vp, vp, i, i, i64, vp, i, i, i,
+                                    vp, vp]
+    L.xdna_paged_append.restype = i
+    L.xdna_paged_attention.argtypes = [vp, i, vp, i64, i, vp, i, i, i64, vp, f, i, vp, vp, vp]
+    L.xdna_paged_attention.restype = i
+    L.xdna_paged_cache_check.argtypes = [vp, vp]
+    L.xdna_paged_cache_check.restype = i
+    L.xdna_rmsnorm_residual_i8.argtypes = [vp, i, i64, vp, i, i64, vp, i, f, i, i, vp, vp, vp, vp, vp]
+    L.xdna_rmsnorm_residual_i8.restype = i
+    L.xdna_logits_process.argtypes = [vp, i, i64, i, i, vp, i, vp, vp, vp, vp, vp, vp, vp, i, vp, vp, i64,
+                                      vp, i64, vp, vp]
+    L.xdna_logits_process.restype = i
+    return L
+
+
+_L = None
+
+
+def _lib():
+    global _L
+    if _L is None:
+        _L = _declare(lib())
+    return _L
+
+
+def _want(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _flat(t, dtype, shape, dev, name):
+    """The address of a contiguous tensor of exactly this type, shape and device (None: NULL)."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name}: want a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}")
+    return t.data_ptr()
+
+
+def _stream(stream, dev):
+    return torch.cuda.current_stream(dev).cuda_stream if stream is None else stream
+
+
+class _on:
+    """The tensors' device as the current one during a call."""
+
+    def __init__(self, dev):
+        self.dev = dev.index
+
+    def __enter__(self):
+        self.was = torch.cuda.current_device()
+        if self.was != self.dev:
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *_):
+        if self.was != self.dev:
+            torch.cuda.set_device(self.was)
+
+
+def rope_table(n_positions, rot_dim, theta=10000.0, device="cuda"):
+    """The rotary table that PagedCache.append takes: [n_positions][rot_dim] f32, a position's
+    rot_dim / 2 cosines, then its sines, of angles position * theta^(-2 i / rot_dim) in 64 bits."""
+    inv = float(theta) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
+    a = torch.arange(n_positions, dtype=torch.float64, device=device)[:, None] * inv
+    return torch.cat([a.cos(), a.sin()], 1).float()
+
+
+class PagedCache:
+    """A paged key-value cache over the caller's pools k and v: tensors [n_pages, n_kv_heads,
+    page_size, head_dim] (or with a leading [n_layers]), bf16, or int8 with k_scale and v_scale
+    f32 of the same shape without head_dim, contiguous.  k and v may be strided views of one kind (the
+    last dimension contiguous).  The pools are kept alive by this object.  Calls on one object run in
+    one stream at a time."""
+
+    def __init__(self, device, k, v, k_scale=None, v_scale=None, max_seqs=256):
+        _want(k.dim() in (4, 5) and k.shape == v.shape and k.stride() == v.stride() and k.dtype is v.dtype,
+              "k and v: want 4 or 5 dimensions and the same shape, strides and type")
+        _want(k.dtype in (torch.bfloat16, torch.int8), f"k: want bf16 or int8, got {k.dtype}")
+        _want(k.is_cuda and k.device == v.device and k.device.index == device.ordinal,
+              f"k and v are not on device {device.ordinal}")
+        _want(k.stride(-1) == 1, "k: the last dimension is not contiguous")
+        i8 = k.dtype is torch.int8
+        _want(i8 == (k_scale is not None) and i8 == (v_scale is not None), "int8 pools, and only they, have scales")
+        five = k if k.dim() == 5 else k[None]
+        c = _PagedConfig(int(i8), five.shape[0], five.shape[1], five.shape[3], five.shape[2], five.shape[4], max_seqs,
+                         k.data_ptr(), v.data_ptr(), *five.stride()[:4],
+                         _flat(k_scale, torch.float32, k.shape[:-1], k.device, "k_scale"),
+                         _flat(v_scale, torch.float32, k.shape[:-1], k.device, "v_scale"))
+        self.handle = None
+        h = _lib().xdna_paged_cache_create(device.handle, C.byref(c))
+        if not h:
+            raise XdnaError(last_error())
+        self.handle, self._keep = h, (k, v, k_scale, v_scale)
+        self.device, self.n_kv_heads, self.head_dim = k.device, five.shape[2], five.shape[4]
+
+    def append(self, q, k, v, tok_seq, tok_pos, block_table, rope=None, interleaved=False, layer=0, q_out=None,
+               stream=None):
+        """Write the rotated keys and the values of len(tok_pos) tokens into the pools and return
+        their rotated queries (q_out, bf16 [n, n_q_heads, head_dim]; None for q None).  q, k, v
+        [n, heads, head_dim], all bf16 or all f32, heads contiguous, tokens at any stride; tok_seq
+        (None: token t is stream t) and tok_pos int32 [n], block_table int32 [n_seqs, width], rope as
+        rope_table makes it (None: no rotation)."""
+        dev, d, n = self.device, self.head_dim, tok_pos.shape[0]
+        src = k.dtype
+        _want(src in _FLOATS, f"k: want bf16 or f32, got {src}")
+        for name, x in (("q", q), ("k", k), ("v", v)):
+            if x is None and name == "q":
+                continue
+            s = x.stride()
+            _want(x.dtype is src and x.device == dev and x.dim() == 3 and x.shape[0] == n and x.shape[2] == d
+                  and s[2] == 1 and (s[1] == d or x.shape[1] == 1),
+                  f"{name}: want {src} [{n}, heads, {d}] on {dev} with contiguous heads")
+        _want(k.shape[1] == self.n_kv_heads == v.shape[1], f"k and v: want {self.n_kv_heads} heads")
+        _want(block_table.dim() == 2 and block_table.dtype is torch.int32 and block_table.stride(1) == 1
+              and block_table.device == dev, "block_table: want int32 [n_seqs, width], rows contiguous")
+        hq = 0
+        if q is not None:
+            hq = q.shape[1]
+            if q_out is None:
+                q_out = torch.empty(n, hq, d, dtype=torch.bfloat16, device=dev)
+        rows = rot = 0
+        if rope is not None:
+            rows, rot = rope.shape
+        if n == 0:
+            return q_out
+        _check(_lib().xdna_paged_append(
+            self.handle, layer, n, hq, src is torch.float32,
+            None if q is None else q.data_ptr(), 0 if q is None else q.stride(0), k.data_ptr(), k.stride(0),
+            v.data_ptr(), v.stride(0), _flat(tok_seq, torch.int32, (n,), dev, "tok_seq"),
+            _flat(tok_pos, torch.int32, (n,), dev, "tok_pos"), block_table.data_ptr(), block_table.shape[0],
+            block_table.shape[1], block_table.stride(0),
+            None if rope is None else _flat(rope, torch.float32, rope.shape, dev, "rope"), rows, rot, interleaved,
+            None if q is None else _flat(q_out, torch.bfloat16, (n, hq, d), dev, "q_out"), _stream(stream, dev)))
+        return q_out
+
+    def attend(self, q, block_table, seq_lens, scale=None, window=0, layer=0, out=None, lse=None, stream=None):
+        """Attention of one new token per stream, q bf16 [n_seqs, n_q_heads, head_dim], over the last
+        `window` (0: all) of its seq_lens[b] positions; scale None: head_dim ** -0.5.  Returns out
+        (bf16, as q); lse (f32 [n_seqs, n_q_heads]) is filled when given."""
+        dev, d, n = self.device, self.head_dim, seq_lens.shape[0]
+        s = q.stride()
+        _want(q.dtype is torch.bfloat16 and q.device == dev and q.dim() == 3 and q.shape[0] == n and q.shape[2] == d
+              and s[2] == 1 and (s[1] == d or q.shape[1] == 1),
+              f"q: want bf16 [{n}, heads, {d}] on {dev} with contiguous heads")
+        _want(block_table.dim() == 2 and block_table.dtype is torch.int32 and block_table.stride(1) == 1
+              and block_table.shape[0] == n and block_table.device == dev,
+              f"block_table: want int32 [{n}, width], rows contiguous")
+        hq = q.shape[1]
+        if out is None:
+            out = torch.empty(n, hq, d, dtype=torch.bfloat16, device=dev)
+        if n == 0:
+            return out
+        _check(_lib().xdna_paged_attention(
+            self.handle, layer, q.data_ptr(), s[0] if n > 1 else hq * d, hq, block_table.data_ptr(), n,
+            block_table.shape[1], block_table.stride(0), _flat(seq_lens, torch.int32, (n,), dev, "seq_lens"),
+            d ** -0.5 if scale is None else scale, window, _flat(out, torch.bfloat16, (n, hq, d), dev, "out"),
+            _flat(lse, torch.float32, (n, hq), dev, "lse"), _stream(stream, dev)))
+        return out
+
+    def check(self, stream=None):
+        """Wait for the stream and raise XdnaError for page ids, positions or streams out of range
+        that calls since the last check met."""
+        _check(_lib().xdna_paged_cache_check(self.handle, _stream(stream, self.device)))
+
+    def close(self):
+        if getattr(self, "handle", None):
+            _lib().xdna_paged_cache_free(self.handle)
+            self.handle = self._keep = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _rows(x, m, d, dev, name):
+    """Row stride of an [m, d] tensor with contiguous rows."""
+    _want(x.dim() == 2 and x.shape[0] == m and x.shape[1] == d and x.dtype in _FLOATS and x.device == dev
+          and (x.stride(1) == 1 or d == 1), f"{name}: want bf16 or f32 [{m}, {d}] on {dev}, rows contiguous")
+    return x.stride(0) if m > 1 else d
+
+
+def rmsnorm_residual_i8(x, gamma, residual=None, eps=1e-6, unit_offset=False, q8=None, scale=None, residual_out=None,
+                        y=None, quantize=True, stream=None):
+    """r = x + residual; y = r / sqrt(mean(r^2) + eps) * gamma (gamma + 1 with unit_offset), as int8
+    rows with scales (y = q8 * scale).  x and residual bf16 or f32 [m, d].  Returns (q8, scale,
+    residual_out): residual_out holds r in residual's type (None without a residual); a given buffer is
+    used, residual itself among them.  `y` (bf16 [m, d]) also takes the unquantised norm;
+    quantize=False leaves q8 and scale out (None)."""
+    _want(x.dim() == 2, "x: want [m, d]")
+    dev, (m, d) = x.device, x.shape
+    xs = _rows(x, m, d, dev, "x")
+    rs = 0
+    if residual is not None:
+        rs = _rows(residual, m, d, dev, "residual")
+        if residual_out is None:
+            residual_out = torch.empty_strided((m, d), (rs, 1), dtype=residual.dtype, device=dev)
+        _want(residual_out.dtype is residual.dtype and _rows(residual_out, m, d, dev, "residual_out") == rs,
+              "residual_out: want the type and row stride of residual")
+    else:
+        _want(residual_out is None, "residual_out without a residual")
+    if quantize:
+        if q8 is None:
+            q8 = torch.empty(m, d, dtype=torch.int8, device=dev)
+        if scale is None:
+            scale = torch.empty(m, dtype=torch.float32, device=dev)
+    else:
+        _want(q8 is None and scale is None, "q8 or scale with quantize=False")
+    if m == 0:
+        return q8, scale, residual_out
+    with _on(dev):
+        _check(_lib().xdna_rmsnorm_residual_i8(
+            x.data_ptr(), x.dtype is torch.float32, xs, None if residual is None else residual.data_ptr(),
+            residual is not None and residual.dtype is torch.float32, rs,
+            _flat(gamma, torch.float32, (d,), dev, "gamma"), unit_offset, eps, m, d,
+            None if residual_out is None else residual_out.data_ptr(),
+            _flat(y, torch.bfloat16, (m, d), dev, "y"), _flat(q8, torch.int8, (m, d), dev, "q8"),
+            _flat(scale, torch.float32, (m,), dev, "scale"), _stream(stream, dev)))
+    return q8, scale, residual_out
+
+
+def process_logits(logits, history=None, history_start=None, n_prompt=None, repetition=None, frequency=None,
+                   presence=None, bias_ids=None, bias=None, bias_start=None, mask=None, out=None, ids=None,
+                   stream=None):
+    """Penalties, biases and mask on logits [b, v] (bf16 or f32), in the order of
+    xdna_logits_process; returns (out f32 [b, v], ids int64 [b]: the greedy next token, -1 where the
+    mask leaves none).  history int32 [total] with history_start int32 [b + 1]; n_prompt int32 [b];
+    repetition, frequency, presence f32 [b]; bias_ids int32, bias f32 [entries] with bias_start int32
+    [b + 1]; mask int32 [b, (v + 31) / 32], bit set: allowed.  out may be logits (f32)."""
+    _want(logits.dim() == 2, "logits: want [b, v]")
+    dev, (b, v) = logits.device, logits.shape
+    ls = _rows(logits, b, v, dev, "logits")
+    if out is None:
+        out = torch.empty(b, v, dtype=torch.float32, device=dev)
+    os_ = _rows(out, b, v, dev, "out")
+    _want(out.dtype is torch.float32, "out: want f32")
+    if ids is None:
+        ids = torch.empty(b, dtype=torch.int64, device=dev)
+    if b == 0:
+        return out, ids
+    i32, f32 = torch.int32, torch.float32
+    _want(history is None or history.dim() == 1, "history: want one dimension")
+    _want(bias is None or bias.dim() == 1, "bias: want one dimension")
+    n = 0 if history is None else history.shape[0]
+    e = 0 if bias is None else bias.shape[0]
+    with _on(dev):
+        _check(_lib().xdna_logits_process(
+            logits.data_ptr(), logits.dtype is f32, ls, b, v, _flat(history, i32, (n,), dev, "history"), n,
+            _flat(history_start, i32, (b + 1,), dev, "history_start"), _flat(n_prompt, i32, (b,), dev, "n_prompt"),
+            _flat(repetition, f32, (b,), dev, "repetition"), _flat(frequency, f32, (b,), dev, "frequency"),
+            _flat(presence, f32, (b,), dev, "presence"), _flat(bias_ids, i32, (e,), dev, "bias_ids"),
+            _flat(bias, f32, (e,), dev, "bias"), e, _flat(bias_start, i32, (b + 1,), dev, "bias_start"),
+            _flat(mask, i32, (b, (v + 31) // 32), dev, "mask"), (v + 31) // 32, out.data_ptr(), os_,
+            _flat(ids, torch.int64, (b,), dev, "ids"), _stream(stream, dev)))
+    return out, ids
