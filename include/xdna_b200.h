@@ -607,14 +607,18 @@ int xdna_rmsnorm_residual_i8(const void *x, int x_f32, int64_t x_stride, const v
  * n_biases are the lengths of history and of bias: offsets are held within them.  Every one of the
  * arrays may be NULL (history with history_start, the bias arrays together).  out [B][V] f32
  * rows out_stride apart (may be logits itself if f32), ids [B] (NULL: none): the id of the
- * largest result, the lowest of equals, NaN never, -1 when nothing is above -inf. */
+ * largest result, the lowest of equals, NaN never, -1 when nothing is above -inf.  workspace:
+ * xdna_logits_workspace(B, V) bytes, 8-byte aligned (NULL without ids).  B <= 65535. */
 int xdna_logits_process(const void *logits, int src_f32, int64_t logits_stride, int B, int V,
                         const int32_t *history, int n_history, const int32_t *history_start,
                         const int32_t *n_prompt, const float *repetition, const float *frequency,
                         const float *presence, const int32_t *bias_ids, const float *bias, int n_biases,
                         const int32_t *bias_start,
                         const uint32_t *mask, int64_t mask_stride, float *out, int64_t out_stride, int64_t *ids,
-                        void *stream);
+                        void *workspace, void *stream);
+/* bytes of device memory that xdna_logits_process needs at `workspace` to give ids (its contents
+ * matter only during the call) */
+size_t xdna_logits_workspace(int B, int V);
 
 
 /* ------------------------------------------------- weight stores (npu-weights arena, npy dirs) */

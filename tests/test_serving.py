@@ -37,13 +37,13 @@ def test_null_and_shape_refusals(S):
     assert norm(M=0) == 0
     logits = lambda **k: L.xdna_logits_process(*{**dict(  # noqa: E731
         x=p, f=1, ls=8, B=2, V=8, h=None, nh=0, hs=None, np=None, rep=None, fr=None, pr=None, bi=None, b=None, nb=0,
-        bs=None, m=None, ms=0, o=p, os=8, ids=p, st=None), **k}.values())
+        bs=None, m=None, ms=0, o=p, os=8, ids=p, ws=p, st=None), **k}.values())
     for bad, why in ((dict(x=None), "null"), (dict(o=None), "null"), (dict(V=0), "V"), (dict(B=-1), "B"),
                      (dict(h=p), "together"), (dict(hs=p), "together"), (dict(rep=p), "history"),
                      (dict(np=p), "history"), (dict(b=p), "together"), (dict(bi=p, b=p), "together"),
                      (dict(ls=7), "stride"), (dict(os=7), "stride"), (dict(m=p, ms=0), "mask_stride"),
                      (dict(nh=-1), "n_history"), (dict(nb=-1), "n_biases"), (dict(f=0), "bf16"),
-                     (dict(os=16), "stride")):
+                     (dict(os=16), "stride"), (dict(ws=None), "workspace"), (dict(B=65536), "65535")):
         assert logits(**bad) == -1 and why in X.last_error(), bad
     assert logits(B=0) == 0
 

@@ -43,8 +43,10 @@ def _declare(L):
     L.xdna_rmsnorm_residual_i8.argtypes = [vp, i, i64, vp, i, i64, vp, i, f, i, i, vp, vp, vp, vp, vp]
     L.xdna_rmsnorm_residual_i8.restype = i
     L.xdna_logits_process.argtypes = [vp, i, i64, i, i, vp, i, vp, vp, vp, vp, vp, vp, vp, i, vp, vp, i64,
-                                      vp, i64, vp, vp]
+                                      vp, i64, vp, vp, vp]
     L.xdna_logits_process.restype = i
+    L.xdna_logits_workspace.argtypes = [i, i]
+    L.xdna_logits_workspace.restype = C.c_size_t
     return L
 
 
@@ -73,24 +75,13 @@ def _flat(t, dtype, shape, dev, name):
     return t.data_ptr()
 
 
+# the raw stream without building a torch.cuda.Stream (2 us of a small call), where torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _stream(stream, dev):
-    return torch.cuda.current_stream(dev).cuda_stream if stream is None else stream
-
-
-class _on:
-    """The tensors' device as the current one during a call."""
-
-    def __init__(self, dev):
-        self.dev = dev.index
-
-    def __enter__(self):
-        self.was = torch.cuda.current_device()
-        if self.was != self.dev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *_):
-        if self.was != self.dev:
-            torch.cuda.set_device(self.was)
+    return _raw_stream(dev.index) if stream is None else stream
 
 
 def rope_table(n_positions, rot_dim, theta=10000.0, device="cuda"):
@@ -99,6 +90,18 @@ def rope_table(n_positions, rot_dim, theta=10000.0, device="cuda"):
     inv = float(theta) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
     a = torch.arange(n_positions, dtype=torch.float64, device=device)[:, None] * inv
     return torch.cat([a.cos(), a.sin()], 1).float()
+
+
+def _is_heads(x, dtype, n, d, dev):
+    """Whether x is [n, heads, d] with contiguous heads."""
+    s, shape = x.stride(), x.shape
+    return (len(s) == 3 and x.dtype is dtype and x.device == dev and shape[0] == n and shape[2] == d and s[2] == 1
+            and (s[1] == d or shape[1] == 1))
+
+
+def _is_table(t, dev):
+    s = t.stride()
+    return len(s) == 2 and t.dtype is torch.int32 and t.device == dev and (s[1] == 1 or t.shape[1] == 1)
 
 
 class PagedCache:
@@ -142,13 +145,10 @@ class PagedCache:
         for name, x in (("q", q), ("k", k), ("v", v)):
             if x is None and name == "q":
                 continue
-            s = x.stride()
-            _want(x.dtype is src and x.device == dev and x.dim() == 3 and x.shape[0] == n and x.shape[2] == d
-                  and s[2] == 1 and (s[1] == d or x.shape[1] == 1),
-                  f"{name}: want {src} [{n}, heads, {d}] on {dev} with contiguous heads")
+            if not _is_heads(x, src, n, d, dev):
+                raise ValueError(f"{name}: want {src} [{n}, heads, {d}] on {dev} with contiguous heads")
         _want(k.shape[1] == self.n_kv_heads == v.shape[1], f"k and v: want {self.n_kv_heads} heads")
-        _want(block_table.dim() == 2 and block_table.dtype is torch.int32 and block_table.stride(1) == 1
-              and block_table.device == dev, "block_table: want int32 [n_seqs, width], rows contiguous")
+        _want(_is_table(block_table, dev), "block_table: want int32 [n_seqs, width], rows contiguous")
         hq = 0
         if q is not None:
             hq = q.shape[1]
@@ -174,20 +174,17 @@ class PagedCache:
         `window` (0: all) of its seq_lens[b] positions; scale None: head_dim ** -0.5.  Returns out
         (bf16, as q); lse (f32 [n_seqs, n_q_heads]) is filled when given."""
         dev, d, n = self.device, self.head_dim, seq_lens.shape[0]
-        s = q.stride()
-        _want(q.dtype is torch.bfloat16 and q.device == dev and q.dim() == 3 and q.shape[0] == n and q.shape[2] == d
-              and s[2] == 1 and (s[1] == d or q.shape[1] == 1),
-              f"q: want bf16 [{n}, heads, {d}] on {dev} with contiguous heads")
-        _want(block_table.dim() == 2 and block_table.dtype is torch.int32 and block_table.stride(1) == 1
-              and block_table.shape[0] == n and block_table.device == dev,
-              f"block_table: want int32 [{n}, width], rows contiguous")
+        if not _is_heads(q, torch.bfloat16, n, d, dev):
+            raise ValueError(f"q: want bf16 [{n}, heads, {d}] on {dev} with contiguous heads")
+        _want(_is_table(block_table, dev) and block_table.shape[0] == n,
+              "block_table: want int32 [n_seqs, width], rows contiguous")
         hq = q.shape[1]
         if out is None:
             out = torch.empty(n, hq, d, dtype=torch.bfloat16, device=dev)
         if n == 0:
             return out
         _check(_lib().xdna_paged_attention(
-            self.handle, layer, q.data_ptr(), s[0] if n > 1 else hq * d, hq, block_table.data_ptr(), n,
+            self.handle, layer, q.data_ptr(), q.stride(0) if n > 1 else hq * d, hq, block_table.data_ptr(), n,
             block_table.shape[1], block_table.stride(0), _flat(seq_lens, torch.int32, (n,), dev, "seq_lens"),
             d ** -0.5 if scale is None else scale, window, _flat(out, torch.bfloat16, (n, hq, d), dev, "out"),
             _flat(lse, torch.float32, (n, hq), dev, "lse"), _stream(stream, dev)))
@@ -212,9 +209,10 @@ class PagedCache:
 
 def _rows(x, m, d, dev, name):
     """Row stride of an [m, d] tensor with contiguous rows."""
-    _want(x.dim() == 2 and x.shape[0] == m and x.shape[1] == d and x.dtype in _FLOATS and x.device == dev
-          and (x.stride(1) == 1 or d == 1), f"{name}: want bf16 or f32 [{m}, {d}] on {dev}, rows contiguous")
-    return x.stride(0) if m > 1 else d
+    s = x.stride()
+    if x.shape != (m, d) or x.dtype not in _FLOATS or x.device != dev or (s[1] != 1 and d > 1):
+        raise ValueError(f"{name}: want bf16 or f32 [{m}, {d}] on {dev}, rows contiguous")
+    return s[0] if m > 1 else d
 
 
 def rmsnorm_residual_i8(x, gamma, residual=None, eps=1e-6, unit_offset=False, q8=None, scale=None, residual_out=None,
@@ -224,7 +222,7 @@ def rmsnorm_residual_i8(x, gamma, residual=None, eps=1e-6, unit_offset=False, q8
     residual_out): residual_out holds r in residual's type (None without a residual); a given buffer is
     used, residual itself among them.  `y` (bf16 [m, d]) also takes the unquantised norm;
     quantize=False leaves q8 and scale out (None)."""
-    _want(x.dim() == 2, "x: want [m, d]")
+    _want(x.dim() == 2 and x.is_cuda, "x: want [m, d] on a GPU")
     dev, (m, d) = x.device, x.shape
     xs = _rows(x, m, d, dev, "x")
     rs = 0
@@ -245,7 +243,10 @@ def rmsnorm_residual_i8(x, gamma, residual=None, eps=1e-6, unit_offset=False, q8
         _want(q8 is None and scale is None, "q8 or scale with quantize=False")
     if m == 0:
         return q8, scale, residual_out
-    with _on(dev):
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            rmsnorm_residual_i8(x, gamma, residual, eps, unit_offset, q8, scale, residual_out, y, quantize, stream)
+    else:
         _check(_lib().xdna_rmsnorm_residual_i8(
             x.data_ptr(), x.dtype is torch.float32, xs, None if residual is None else residual.data_ptr(),
             residual is not None and residual.dtype is torch.float32, rs,
@@ -264,7 +265,7 @@ def process_logits(logits, history=None, history_start=None, n_prompt=None, repe
     mask leaves none).  history int32 [total] with history_start int32 [b + 1]; n_prompt int32 [b];
     repetition, frequency, presence f32 [b]; bias_ids int32, bias f32 [entries] with bias_start int32
     [b + 1]; mask int32 [b, (v + 31) / 32], bit set: allowed.  out may be logits (f32)."""
-    _want(logits.dim() == 2, "logits: want [b, v]")
+    _want(logits.dim() == 2 and logits.is_cuda, "logits: want [b, v] on a GPU")
     dev, (b, v) = logits.device, logits.shape
     ls = _rows(logits, b, v, dev, "logits")
     if out is None:
@@ -278,9 +279,14 @@ def process_logits(logits, history=None, history_start=None, n_prompt=None, repe
     i32, f32 = torch.int32, torch.float32
     _want(history is None or history.dim() == 1, "history: want one dimension")
     _want(bias is None or bias.dim() == 1, "bias: want one dimension")
+    work = torch.empty(_lib().xdna_logits_workspace(b, v) // 8, dtype=torch.int64, device=dev)
     n = 0 if history is None else history.shape[0]
     e = 0 if bias is None else bias.shape[0]
-    with _on(dev):
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            process_logits(logits, history, history_start, n_prompt, repetition, frequency, presence, bias_ids, bias,
+                           bias_start, mask, out, ids, stream)
+    else:
         _check(_lib().xdna_logits_process(
             logits.data_ptr(), logits.dtype is f32, ls, b, v, _flat(history, i32, (n,), dev, "history"), n,
             _flat(history_start, i32, (b + 1,), dev, "history_start"), _flat(n_prompt, i32, (b,), dev, "n_prompt"),
@@ -288,5 +294,5 @@ def process_logits(logits, history=None, history_start=None, n_prompt=None, repe
             _flat(presence, f32, (b,), dev, "presence"), _flat(bias_ids, i32, (e,), dev, "bias_ids"),
             _flat(bias, f32, (e,), dev, "bias"), e, _flat(bias_start, i32, (b + 1,), dev, "bias_start"),
             _flat(mask, i32, (b, (v + 31) // 32), dev, "mask"), (v + 31) // 32, out.data_ptr(), os_,
-            _flat(ids, torch.int64, (b,), dev, "ids"), _stream(stream, dev)))
+            _flat(ids, torch.int64, (b,), dev, "ids"), work.data_ptr(), _stream(stream, dev)))
     return out, ids
