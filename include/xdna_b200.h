@@ -608,7 +608,7 @@ int xdna_rmsnorm_residual_i8(const void *x, int x_f32, int64_t x_stride, const v
  * arrays may be NULL (history with history_start, the bias arrays together).  out [B][V] f32
  * rows out_stride apart (may be logits itself if f32), ids [B] (NULL: none): the id of the
  * largest result, the lowest of equals, NaN never, -1 when nothing is above -inf.  workspace:
- * xdna_logits_workspace(B, V) bytes, 8-byte aligned (NULL without ids).  B <= 65535. */
+ * xdna_logits_workspace(B, V) bytes, 8-byte aligned (NULL without ids, or when that is 0).  B <= 65535. */
 int xdna_logits_process(const void *logits, int src_f32, int64_t logits_stride, int B, int V,
                         const int32_t *history, int n_history, const int32_t *history_start,
                         const int32_t *n_prompt, const float *repetition, const float *frequency,

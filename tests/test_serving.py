@@ -43,7 +43,7 @@ def test_null_and_shape_refusals(S):
                      (dict(np=p), "history"), (dict(b=p), "together"), (dict(bi=p, b=p), "together"),
                      (dict(ls=7), "stride"), (dict(os=7), "stride"), (dict(m=p, ms=0), "mask_stride"),
                      (dict(nh=-1), "n_history"), (dict(nb=-1), "n_biases"), (dict(f=0), "bf16"),
-                     (dict(os=16), "stride"), (dict(ws=None), "workspace"), (dict(B=65536), "65535")):
+                     (dict(os=16), "stride"), (dict(ws=None, B=1, V=200000, ls=200000, os=200000), "workspace"), (dict(B=65536), "65535")):
         assert logits(**bad) == -1 and why in X.last_error(), bad
     assert logits(B=0) == 0
 

@@ -213,96 +213,240 @@ struct LogitsArgs {
     const float *bias;
     const uint32_t *mask;
     float *out;
-    unsigned long long *best;                             // [B][chunks], NULL: no id wanted
+    int64_t *ids;
+    unsigned long long *best;                             // [B][chunks] where the chunks do not meet in a cluster
 };
 
-// x with its id as one number that is larger for the larger x, of equals for the lower id; 0: none
-__device__ __forceinline__ unsigned long long choice(float x, int id) {
+// a float's bits as an unsigned that orders alike (-0 as 0); -inf and NaN: 0, below every other
+__device__ __forceinline__ unsigned ordered(float x) {
     const unsigned u = __float_as_uint(x == 0.0f ? 0.0f : x);
-    const unsigned key = u & 0x80000000u ? ~u : u | 0x80000000u;
-    return x > -INFINITY ? ((unsigned long long)key << 32) | (0xffffffffu - (unsigned)id) : 0ull;
+    return x > -INFINITY ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;
 }
-__device__ __forceinline__ unsigned long long largest(unsigned long long k) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
-        k = other > k ? other : k;
-    }
-    return k;
+// a value and its id as one number: larger for the larger value, of equals for the lower id; 0: none
+__device__ __forceinline__ unsigned long long choice(unsigned key, int id) {
+    return key ? ((unsigned long long)key << 32) | (0xffffffffu - (unsigned)id) : 0ull;
 }
 
-// One CTA per row and chunk of 512 E ids.  A logit is read once into a register before anything else, so
-// that its latency passes under the counting: the chunk's counts and bias entries are built in
-// shared memory from the row's history and bias list (integer atomics, so in any order), which every
-// chunk of the row scans.  4 + 4 bytes an id in f32: HBM bounds it.  The chunk's best id goes to the
-// workspace, from which choose_kernel takes the row's.
-constexpr int kLogitsThreads = 512;
-template <typename T, int E>
-__global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const LogitsArgs a) {
-    constexpr int kChunk = kLogitsThreads * E;
-    extern __shared__ unsigned smem[];
-    __shared__ unsigned long long red[kLogitsThreads / 32];
-    unsigned *count = smem;                               // generated occurrences; bit 31: seen at all
-    int *entry = reinterpret_cast<int *>(smem + (a.hist ? kChunk : 0));   // 1 + the id's last bias entry
-    const int64_t b = blockIdx.y;
-    const int tid = threadIdx.x, v0 = blockIdx.x * kChunk, nv = min(kChunk, a.V - v0);
-    const T *x = static_cast<const T *>(a.logits) + b * a.stride + v0;
-    float y[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int i = e * kLogitsThreads + tid;
-        y[e] = i < nv ? to_f32(x[i]) : -INFINITY;
+// One CTA per row and chunk of 512 P W ids; 4 + 4 bytes an id in f32, so HBM bounds it as long as an id
+// costs few instructions.
+// * A thread takes P pieces of W ids.  W = 4: one 16-byte access, with chunks laid from the row's
+//   preceding 16-byte boundary where rows start off one; W = 1 where logits and out lie differently.
+// * Logits, mask bits and list entries are loaded into registers before they are needed, so that
+//   their latencies pass together; every chunk of a row scans the row's lists.
+// * The chunk's counts and bias entries lie in shared memory (integer atomics, so in any order), with a
+//   bit per touched id.  The touched ids' penalties and biases are worked out first, from the
+//   bits, and their results put where the counts were; then every id is taken from its register or
+//   from there, masked, stored and compared.
+// * The best ids of a row's chunks meet in a cluster (kCluster: the row's CTAs are one), whose first
+//   CTA writes the row's, or in the workspace, from which choose_kernel takes it.
+constexpr int kLogitsThreads = 512, kLogitsWarps = kLogitsThreads / 32, kMaxCluster = 8;
+
+template <int W>
+__device__ __forceinline__ void load_ids(const float *x, float *y) {
+    if (W == 4) {
+        const float4 v = __ldcs(reinterpret_cast<const float4 *>(x));
+        y[0] = v.x; y[1] = v.y; y[2] = v.z; y[3] = v.w;
+    } else {
+        y[0] = *x;
     }
-    const int h0 = a.hist ? max(0, a.hist_start[b]) : 0, h1 = a.hist ? min(a.n_hist, a.hist_start[b + 1]) : 0;
-    const int64_t gen = (int64_t)h0 + (a.n_prompt ? a.n_prompt[b] : 0);
-    const int e0 = a.bias ? max(0, a.bias_start[b]) : 0, e1 = a.bias ? min(a.n_bias, a.bias_start[b + 1]) : 0;
-    if (a.hist || a.bias) {
-        const int words = kChunk * ((a.hist ? 1 : 0) + (a.bias ? 1 : 0));
-        for (int i = tid; i < words / 4; i += kLogitsThreads) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
+}
+template <int W>
+__device__ __forceinline__ void load_ids(const __nv_bfloat16 *x, float *y) {
+    if (W == 4) {
+        const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(x));
+        y[0] = xdna::bf16lo(v.x); y[1] = xdna::bf16hi(v.x); y[2] = xdna::bf16lo(v.y); y[3] = xdna::bf16hi(v.y);
+    } else {
+        y[0] = __bfloat162float(*x);
+    }
+}
+
+template <typename T, int P, int W, bool kCluster>
+__global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const LogitsArgs a) {
+    constexpr int kChunk = kLogitsThreads * P * W, kAhead = 8, kBits = P * W;   // kBits: touched bits a thread works out
+    constexpr unsigned kPiece = (1u << W) - 1;
+    extern __shared__ __align__(16) unsigned smem[];
+    // bit i: place i is in the history (any: in the history or the bias list)
+    __shared__ unsigned seen[kChunk / 32], any[kChunk / 32];
+    __shared__ unsigned key_of[kLogitsWarps], id_of[kLogitsWarps];
+    __shared__ unsigned long long of_rank[kMaxCluster];
+    unsigned *count = smem;                               // generated occurrences, then the touched ids' results
+    int *entry = reinterpret_cast<int *>(smem + kChunk);  // 1 + the id's last bias entry
+    const int64_t b = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    if constexpr (kCluster) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+    // the chunk's place i is id first + i, live for lo <= i < hi
+    const int shift = W == 4 ? (int)((reinterpret_cast<uintptr_t>(a.out + b * a.out_stride) / 4) % 4) : 0;
+    const int first = blockIdx.x * kChunk - shift, lo = max(0, -first), hi = min(kChunk, a.V - first);
+    const bool full = lo == 0 && hi == kChunk;
+    const T *x = static_cast<const T *>(a.logits) + b * a.stride + first;
+    float *out = a.out + b * a.out_stride + first;
+    auto place_of = [&](int p) { return (p * kLogitsThreads + tid) * W; };
+    float y[P][W];
+    unsigned allowed = 0xffffffffu;                       // bit p W + w
+    const uint32_t *mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
+    if (full) {
+#pragma unroll
+        for (int p = 0; p < P; p++) load_ids<W>(x + place_of(p), y[p]);
+    } else {
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const int i = place_of(p) + w;
+                y[p][w] = i >= lo && i < hi ? to_f32(x[i]) : -INFINITY;
+            }
+    }
+    if (mask && full && shift == 0) {
+        allowed = 0;
+#pragma unroll
+        for (int p = 0; p < P; p++) allowed |= ((mask[(first + place_of(p)) / 32] >> (place_of(p) % 32)) & kPiece) << (p * W);
+    } else if (mask) {
+        allowed = 0;
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const int i = place_of(p) + w;
+                if (i >= lo && i < hi) allowed |= ((mask[(first + i) / 32] >> ((first + i) % 32)) & 1u) << (p * W + w);
+            }
+    }
+    const bool lists = a.hist || a.bias;
+    if (lists) {
+        const int h0 = a.hist ? max(0, a.hist_start[b]) : 0, h1 = a.hist ? min(a.n_hist, a.hist_start[b + 1]) : 0;
+        const int gen = a.n_prompt ? min(max(0, a.n_prompt[b]), 0x7fffffff - h0) + h0 : h0;
+        const int e0 = a.bias ? max(0, a.bias_start[b]) : 0, e1 = a.bias ? min(a.n_bias, a.bias_start[b + 1]) : 0;
+        const float rep = a.rep ? a.rep[b] : 1.0f, freq = a.freq ? a.freq[b] : 0.0f, pres = a.pres ? a.pres[b] : 0.0f;
+        int biased = e1 - e0 > tid ? a.bias_ids[e0 + tid] : -1;
+        int ids[kAhead];
+        auto ahead = [&](int j0) {
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) ids[k] = h1 - j0 > k * kLogitsThreads + tid ? a.hist[j0 + k * kLogitsThreads + tid] : -1;
+        };
+        if (h0 < h1) ahead(h0);
+        uint4 *zero = reinterpret_cast<uint4 *>(smem) + tid;
+#pragma unroll
+        for (int i = 0; i < kChunk / 4 / kLogitsThreads; i++) zero[i * kLogitsThreads] = make_uint4(0, 0, 0, 0);
+        if (a.bias) {
+#pragma unroll
+            for (int i = 0; i < kChunk / 4 / kLogitsThreads; i++) zero[kChunk / 4 + i * kLogitsThreads] = make_uint4(0, 0, 0, 0);
+        }
+        if (tid < kChunk / 32) seen[tid] = any[tid] = 0;
         __syncthreads();
-        for (int j = h0 + tid; j < h1; j += kLogitsThreads) {
-            const unsigned i = (unsigned)a.hist[j] - (unsigned)v0;
-            if (i < (unsigned)nv) {
-                atomicOr(&count[i], 0x80000000u);
-                if (j >= gen) atomicAdd(&count[i], 1u);
+        // an id of the chunk: id_lo <= id < id_lo + span, as unsigned, which leaves negative ids out
+        const unsigned id_lo = (unsigned)(first + lo), span = (unsigned)max(0, hi - lo);
+        for (int j0 = h0; j0 < h1;) {
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                if ((unsigned)ids[k] - id_lo < span) {
+                    const int i = ids[k] - first;
+                    atomicOr(&seen[i / 32], 1u << (i % 32));
+                    if (j0 + k * kLogitsThreads + tid >= gen) atomicAdd(&count[i], 1u);
+                }
+            }
+            if (h1 - j0 <= kAhead * kLogitsThreads) break;
+            j0 += kAhead * kLogitsThreads;
+            ahead(j0);
+        }
+        for (int j = tid; j < e1 - e0;) {
+            if ((unsigned)biased - id_lo < span) {
+                const int i = biased - first;
+                atomicOr(&any[i / 32], 1u << (i % 32));
+                atomicMax(&entry[i], j + 1);
+            }
+            if (e1 - e0 - j <= kLogitsThreads) break;
+            j += kLogitsThreads;
+            biased = a.bias_ids[e0 + j];
+        }
+        __syncthreads();
+        // ---- touched ids: a thread works out kBits neighbouring places
+        const int from = tid * kBits;
+        const unsigned in_hist = (seen[from / 32] >> (from % 32)) & ((1u << kBits) - 1);
+        for (unsigned left = in_hist | ((any[from / 32] >> (from % 32)) & ((1u << kBits) - 1)); left; left &= left - 1) {
+            const int k = __ffs(left) - 1, i = from + k;
+            float z = to_f32(x[i]);
+            if (a.rep && ((in_hist >> k) & 1u)) z = z > 0.0f ? __fdiv_rn(z, rep) : __fmul_rn(z, rep);
+            const unsigned n = count[i];
+            if (n) z = __fsub_rn(__fsub_rn(z, __fmul_rn((float)n, freq)), pres);
+            if (a.bias && entry[i]) z = __fadd_rn(z, a.bias[e0 + entry[i] - 1]);
+            count[i] = __float_as_uint(z);
+        }
+        __syncthreads();
+    }
+    // ---- every id
+    float top = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+        const int i = place_of(p);
+        if (lists) {
+            const unsigned hit = ((seen[i / 32] | any[i / 32]) >> (i % 32)) & kPiece;
+            if (hit) {
+                float z[W];
+                if constexpr (W == 4) {
+                    const float4 v = *reinterpret_cast<const float4 *>(count + i);
+                    z[0] = v.x; z[1] = v.y; z[2] = v.z; z[3] = v.w;
+                } else {
+                    z[0] = __uint_as_float(count[i]);
+                }
+#pragma unroll
+                for (int w = 0; w < W; w++) y[p][w] = (hit >> w) & 1u ? z[w] : y[p][w];
             }
         }
-        for (int j = e0 + tid; j < e1; j += kLogitsThreads) {
-            const unsigned i = (unsigned)a.bias_ids[j] - (unsigned)v0;
-            if (i < (unsigned)nv) atomicMax(&entry[i], j - e0 + 1);
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            if (!((allowed >> (p * W + w)) & 1u)) y[p][w] = -INFINITY;
+            top = fmaxf(top, y[p][w]);
+        }
+        if (W == 4 && full) {
+            *reinterpret_cast<float4 *>(out + i) = make_float4(y[p][0], y[p][1 % W], y[p][2 % W], y[p][3 % W]);
+        } else {
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                if (i + w >= lo && i + w < hi) out[i + w] = y[p][w];
+        }
+    }
+    // ---- the chunk's choice: the largest value of all, then the lowest place that has it
+    unsigned long long best = 0;
+    if (a.ids) {
+        const unsigned key = __reduce_max_sync(0xffffffffu, ordered(top));
+        int at = 0x7fffffff;
+        if (ordered(top) == key) {
+#pragma unroll
+            for (int p = P - 1; p >= 0; p--)
+#pragma unroll
+                for (int w = W - 1; w >= 0; w--)
+                    if (y[p][w] == top) at = place_of(p) + w;
+        }
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) {
+            key_of[warp] = key;
+            id_of[warp] = key ? (unsigned)(first + at) : 0xffffffffu;
         }
         __syncthreads();
-    }
-    const float rep = a.rep ? a.rep[b] : 1.0f, freq = a.freq ? a.freq[b] : 0.0f, pres = a.pres ? a.pres[b] : 0.0f;
-    float *out = a.out + b * a.out_stride + v0;
-    float best = -INFINITY;
-    int at = 0;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int i = e * kLogitsThreads + tid;
-        if (i >= nv) break;
-        const unsigned n = a.hist ? count[i] : 0u;
-        if (n) {
-            const unsigned g = n & 0x7fffffffu;
-            if (a.rep) y[e] = y[e] > 0.0f ? __fdiv_rn(y[e], rep) : __fmul_rn(y[e], rep);
-            if (g) y[e] = __fsub_rn(__fsub_rn(y[e], __fmul_rn((float)g, freq)), pres);
-        }
-        if (a.bias && entry[i]) y[e] = __fadd_rn(y[e], a.bias[e0 + entry[i] - 1]);
-        // a warp's 32 ids share a word
-        if (a.mask && !((a.mask[b * a.mask_stride + (v0 + i) / 32] >> (tid % 32)) & 1u)) y[e] = -INFINITY;
-        out[i] = y[e];
-        if (y[e] > best) {                                // ids ascend: of equals the first stays
-            best = y[e];
-            at = v0 + i;
+        if (warp == 0) {
+            const unsigned mine = lane < kLogitsWarps ? key_of[lane] : 0u;
+            const unsigned all = __reduce_max_sync(0xffffffffu, mine);
+            const unsigned id = __reduce_min_sync(0xffffffffu, lane < kLogitsWarps && mine == all ? id_of[lane] : 0xffffffffu);
+            best = choice(all, (int)id);
         }
     }
-    if (!a.best) return;
-    unsigned long long k = largest(choice(best, at));
-    if (tid % 32 == 0) red[tid / 32] = k;
-    __syncthreads();
-    if (tid >= 32) return;
-    k = largest(tid < kLogitsThreads / 32 ? red[tid] : 0ull);
-    if (tid == 0) a.best[b * gridDim.x + blockIdx.x] = k;
+    if constexpr (kCluster) {
+        // every CTA of the cluster has started (the barrier's first phase): the first one's memory is
+        // there; its second phase says that all have written
+        const unsigned rank = blockIdx.x;
+        asm volatile("barrier.cluster.wait;" ::: "memory");
+        if (tid == 0) {
+            uint32_t to;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(xdna::smem_u32(&of_rank[rank])));
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(best) : "memory");
+        }
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+        if (rank || tid || !a.ids) return;
+        for (unsigned r = 1; r < gridDim.x; r++) best = max(best, of_rank[r]);
+        a.ids[b] = best ? (int64_t)(0xffffffffu - (unsigned)best) : -1;
+    } else if (a.ids && tid == 0) {
+        a.best[b * gridDim.x + blockIdx.x] = best;
+    }
 }
 
 // one warp per row: the best of its chunks
@@ -316,33 +460,66 @@ __global__ void __launch_bounds__(128) choose_kernel(const unsigned long long *b
         const unsigned long long other = best[b * chunks + c];
         k = other > k ? other : k;
     }
-    k = largest(k);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
     if (lane == 0) ids[b] = k ? (int64_t)(0xffffffffu - (unsigned)k) : -1;
 }
 
-constexpr int kFewestPerThread = 4, kMostPerThread = 16;
+// ids per thread: with 4, a chunk of 2048 ids, 25 CTAs for a row of 50k; with 16, 8192
+constexpr int kFewPerThread = 4, kManyPerThread = 16;
+constexpr int chunks_of(int64_t ids, int per_thread) {
+    return (int)((ids + kLogitsThreads * per_thread - 1) / (kLogitsThreads * per_thread));
+}
 
-template <typename T, int E>
-cudaError_t launch_logits(const LogitsArgs &a, int B, int64_t *ids, cudaStream_t st) {
-    constexpr int kChunk = kLogitsThreads * E;
-    const int chunks = (a.V + kChunk - 1) / kChunk;
-    const size_t smem = (size_t)kChunk * 4 * ((a.hist ? 1 : 0) + (a.bias ? 1 : 0));
-    if (smem > 48 * 1024)
-        if (cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, E>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))
+template <typename T, int P, int W, bool kCluster>
+cudaError_t launch_logits(const LogitsArgs &a, int B, int64_t places, cudaStream_t st) {
+    const int chunks = chunks_of(places, P * W);
+    const size_t smem = a.hist || a.bias ? (size_t)kLogitsThreads * P * W * 4 * (a.bias ? 2 : 1) : 0;
+    if (smem > 40 * 1024)
+        if (cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, P, W, kCluster>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))
             return e;
-    logits_kernel<T, E><<<dim3(chunks, B), kLogitsThreads, smem, st>>>(a);
-    if (cudaError_t e = cudaGetLastError()) return e;
-    if (!ids) return cudaSuccess;
     cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(chunks, B);
+    cfg.blockDim = dim3(kLogitsThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    cfg.attrs = &attr;
+    if (kCluster) {
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim = {(unsigned)chunks, 1, 1};
+        cfg.numAttrs = 1;
+    }
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, logits_kernel<T, P, W, kCluster>, a)) return e;
+    if (kCluster || !a.ids) return cudaSuccess;
     cfg.gridDim = dim3((B + 3) / 4);
     cfg.blockDim = dim3(128);
-    cfg.stream = st;
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &early;
+    cfg.dynamicSmemBytes = 0;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, choose_kernel, (const unsigned long long *)a.best, chunks, B, ids);
+    return cudaLaunchKernelEx(&cfg, choose_kernel, (const unsigned long long *)a.best, chunks, B, a.ids);
+}
+template <typename T, int E, bool kCluster>
+cudaError_t launch_logits(const LogitsArgs &a, int B, bool wide, int64_t places, cudaStream_t st) {
+    return wide ? launch_logits<T, E / 4, 4, kCluster>(a, B, places, st) : launch_logits<T, E, 1, kCluster>(a, B, a.V, st);
+}
+
+// A row of up to 8 chunks is one cluster, small chunks first; a longer one takes the large chunks, or
+// the small ones while the large do not fill the GPU.
+template <typename T>
+cudaError_t launch_logits(const LogitsArgs &a, int B, cudaStream_t st) {
+    // wide accesses need logits and out of a row to lie alike against 4 elements; rows that start off
+    // such a boundary take up to 3 places before their first id
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.logits) / sizeof(T), o = reinterpret_cast<uintptr_t>(a.out) / 4;
+    const bool wide = (x - o) % 4 == 0 && (B == 1 || (a.stride - a.out_stride) % 4 == 0);
+    const int64_t places = (int64_t)a.V + (o % 4 || (B > 1 && a.out_stride % 4) ? 3 : 0);
+    const int few = chunks_of(places, kFewPerThread), many = chunks_of(places, kManyPerThread);
+    if (few <= kMaxCluster) return launch_logits<T, kFewPerThread, true>(a, B, wide, places, st);
+    if (many <= kMaxCluster) return launch_logits<T, kManyPerThread, true>(a, B, wide, places, st);
+    if ((int64_t)B * many < 148) return launch_logits<T, kFewPerThread, false>(a, B, wide, places, st);
+    return launch_logits<T, kManyPerThread, false>(a, B, wide, places, st);
 }
 
 }  // namespace
@@ -375,8 +552,8 @@ int xdna_rmsnorm_residual_i8(const void *x, int x_f32, int64_t x_stride, const v
 }
 
 size_t xdna_logits_workspace(int B, int V) {
-    constexpr int kChunk = kLogitsThreads * kFewestPerThread;
-    return B > 0 && V > 0 ? (size_t)B * (((size_t)V + kChunk - 1) / kChunk) * 8 : 0;
+    if (B < 1 || V < 1 || chunks_of((int64_t)V + 3, kManyPerThread) <= kMaxCluster) return 0;
+    return (size_t)B * chunks_of((int64_t)V + 3, kFewPerThread) * 8;
 }
 int xdna_logits_process(const void *logits, int src_f32, int64_t logits_stride, int B, int V,
                         const int32_t *history, int n_history, const int32_t *history_start,
@@ -397,17 +574,14 @@ int xdna_logits_process(const void *logits, int src_f32, int64_t logits_stride, 
     if (out == logits && (!src_f32 || (B > 1 && out_stride != logits_stride)))
         return fail(me + "out on bf16 logits, or on logits of another stride");
     if (B > 65535) return fail(me + "more than 65535 rows");
-    if (ids && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 8)) return fail(me + "ids need a workspace, 8-byte aligned");
+    if (ids && xdna_logits_workspace(B, V) && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 8))
+        return fail(me + "ids need a workspace, 8-byte aligned");
     if (B == 0) return 0;
     LogitsArgs a{logits, logits_stride, out_stride, mask_stride, V, n_history, n_biases, history, history_start, n_prompt,
                  repetition, frequency, presence, bias_ids, bias_start, bias, mask, out,
-                 ids ? static_cast<unsigned long long *>(workspace) : nullptr};
+                 ids, static_cast<unsigned long long *>(workspace)};
     auto st = static_cast<cudaStream_t>(stream);
-    // few rows: smaller chunks, until there is one for every SM
-    const bool few = (int64_t)B * ((V + 8191) / 8192) < 148;
-    const cudaError_t e =
-        src_f32 ? (few ? launch_logits<float, kFewestPerThread>(a, B, ids, st) : launch_logits<float, kMostPerThread>(a, B, ids, st))
-                : (few ? launch_logits<__nv_bfloat16, kFewestPerThread>(a, B, ids, st) : launch_logits<__nv_bfloat16, kMostPerThread>(a, B, ids, st));
+    const cudaError_t e = src_f32 ? launch_logits<float>(a, B, st) : launch_logits<__nv_bfloat16>(a, B, st);
     return ck(e, "xdna_logits_process") ? 0 : -1;
 }
 

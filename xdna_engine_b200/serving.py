@@ -69,7 +69,7 @@ def _flat(t, dtype, shape, dev, name):
     """The address of a contiguous tensor of exactly this type, shape and device (None: NULL)."""
     if t is None:
         return None
-    if t.dtype is not dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev.index or not t.is_contiguous():
         raise ValueError(f"{name}: want a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}")
     return t.data_ptr()
@@ -95,13 +95,13 @@ def rope_table(n_positions, rot_dim, theta=10000.0, device="cuda"):
 def _is_heads(x, dtype, n, d, dev):
     """Whether x is [n, heads, d] with contiguous heads."""
     s, shape = x.stride(), x.shape
-    return (len(s) == 3 and x.dtype is dtype and x.device == dev and shape[0] == n and shape[2] == d and s[2] == 1
+    return (len(s) == 3 and x.dtype is dtype and x.get_device() == dev.index and shape[0] == n and shape[2] == d and s[2] == 1
             and (s[1] == d or shape[1] == 1))
 
 
 def _is_table(t, dev):
     s = t.stride()
-    return len(s) == 2 and t.dtype is torch.int32 and t.device == dev and (s[1] == 1 or t.shape[1] == 1)
+    return len(s) == 2 and t.dtype is torch.int32 and t.get_device() == dev.index and (s[1] == 1 or t.shape[1] == 1)
 
 
 class PagedCache:
@@ -210,7 +210,7 @@ class PagedCache:
 def _rows(x, m, d, dev, name):
     """Row stride of an [m, d] tensor with contiguous rows."""
     s = x.stride()
-    if x.shape != (m, d) or x.dtype not in _FLOATS or x.device != dev or (s[1] != 1 and d > 1):
+    if x.shape != (m, d) or x.dtype not in _FLOATS or x.get_device() != dev.index or (s[1] != 1 and d > 1):
         raise ValueError(f"{name}: want bf16 or f32 [{m}, {d}] on {dev}, rows contiguous")
     return s[0] if m > 1 else d
 
@@ -279,7 +279,8 @@ def process_logits(logits, history=None, history_start=None, n_prompt=None, repe
     i32, f32 = torch.int32, torch.float32
     _want(history is None or history.dim() == 1, "history: want one dimension")
     _want(bias is None or bias.dim() == 1, "bias: want one dimension")
-    work = torch.empty(_lib().xdna_logits_workspace(b, v) // 8, dtype=torch.int64, device=dev)
+    work = _lib().xdna_logits_workspace(b, v)
+    work = torch.empty(work, dtype=torch.uint8, device=dev) if work else None
     n = 0 if history is None else history.shape[0]
     e = 0 if bias is None else bias.shape[0]
     if dev.index != torch.cuda.current_device():
@@ -294,5 +295,6 @@ def process_logits(logits, history=None, history_start=None, n_prompt=None, repe
             _flat(presence, f32, (b,), dev, "presence"), _flat(bias_ids, i32, (e,), dev, "bias_ids"),
             _flat(bias, f32, (e,), dev, "bias"), e, _flat(bias_start, i32, (b + 1,), dev, "bias_start"),
             _flat(mask, i32, (b, (v + 31) // 32), dev, "mask"), (v + 31) // 32, out.data_ptr(), os_,
-            _flat(ids, torch.int64, (b,), dev, "ids"), work.data_ptr(), _stream(stream, dev)))
+            _flat(ids, torch.int64, (b,), dev, "ids"), None if work is None else work.data_ptr(),
+            _stream(stream, dev)))
     return out, ids
