@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -475,10 +476,17 @@ template <typename T, int P, int W, bool kCluster>
 cudaError_t launch_logits(const LogitsArgs &a, int B, int64_t places, cudaStream_t st) {
     const int chunks = chunks_of(places, P * W);
     const size_t smem = a.hist || a.bias ? (size_t)kLogitsThreads * P * W * 4 * (a.bias ? 2 : 1) : 0;
-    if (smem > 40 * 1024)
-        if (cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, P, W, kCluster>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))
-            return e;
+    if (smem > 40 * 1024) {
+        static std::atomic<uint64_t> allowed{0};          // the devices (of the first 64) on which it has been raised
+        int dev = 0;
+        if (cudaError_t e = cudaGetDevice(&dev)) return e;
+        if (dev > 63 || !(allowed.load() >> dev & 1)) {
+            if (cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, P, W, kCluster>,
+                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, kLogitsThreads * P * W * 8))
+                return e;
+            if (dev <= 63) allowed.fetch_or(1ull << dev);
+        }
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(chunks, B);
     cfg.blockDim = dim3(kLogitsThreads);

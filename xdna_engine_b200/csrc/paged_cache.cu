@@ -2,11 +2,13 @@
 // and attention of one new token per stream over it (xdna_paged_*, include/xdna_b200.h).
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <algorithm>
 #include <cstdint>
 #include <new>
 #include <string>
+#include <type_traits>
 
 #include "../../include/xdna_b200.h"
 #include "ptx.cuh"
@@ -24,11 +26,10 @@ struct XdnaPagedCache {
     XdnaPagedCacheConfig cfg{};
     int sms = 0;
     unsigned *status = nullptr;
-    // parts of units that several CTAs share, see the attention kernel; split grows with the units
-    // (streams x K/V heads x head groups) that max_seqs allows: at most kMaxGroups groups a head
+    // parts of units that several CTAs share and counts of those that are there, see the attention kernel
     float *part_o = nullptr;
     float2 *part_ml = nullptr;
-    int2 *split = nullptr;
+    int *arrived = nullptr;
 };
 
 namespace {
@@ -225,16 +226,24 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 // Work split.  A unit is (stream, K/V head, group of up to 8 NT query heads); its keys are cut into
 // tiles of 16 keys per warp.  All units' tiles, laid end to end, are dealt to the CTAs in equal
 // contiguous shares, whatever the streams' lengths; a CTA walks its share unit by unit.  A unit
-// that lies in one CTA is written at once; one that a share's border cuts leaves its
-// (max, sum, unnormalised o) in the workspace, and join_kernel adds the parts in CTA order.
+// that lies in one CTA is written at once; of one that shares' borders cut, each CTA leaves its
+// (max, sum, unnormalised o) in the workspace, and the last of every 16 neighbours to do so adds
+// theirs, in CTA order whoever is last, until one is left: no CTA waits, no second launch.  A fence, an atomic and a part's way through L2 take about 3 us, as long as some 4 tiles: a small call
+// gets fewer CTAs, so that a unit has no more than 16 parts, or exactly as many a unit.
 //
-// Inside a CTA each warp runs alone: its own ring of cp.async stages (16 keys' K and V rows), its own
-// running maximum and sum, no barrier until the unit's end, where the warps' parts are added.
-// S^T = K q^T and o^T += V^T p^T are m16n8k16 products with the keys (the components) in the 16-row
-// operand, so that 8 query heads fill the 8 columns and fewer heads waste nothing but columns.
-// The weights p are used as two bf16 terms (16 bits), which keeps the output's error that of its own
-// rounding.  Keys past the end, before the window or on a bad page are zero-filled in shared
-// memory and masked: what lies in the pool there is not read.
+// Inside a CTA each warp runs alone: its own ring of cp.async stages (16 keys' K and V rows), which
+// runs on over the share's units without a break, its own running maximum and sum, no barrier
+// until a unit's end, where the warps' parts are added.  S^T = K q^T and o^T += V^T p^T are m16n8k16
+// products with the keys (the components) in the 16-row operand, so that 8 query heads fill the 8
+// columns and fewer heads waste nothing but columns.  The weights p are used as two 16-bit terms,
+// which keeps the output's error that of its own rounding.  Keys past the end, before the window or on
+// a bad page are zero-filled in shared memory and masked: what lies in the pool there is not read.
+//
+// bf16 pools: bf16 products.  int8 pools: fp16 products, to which a whole number converts in 5/4
+// instructions (bf16: 2), at 4 KB a step of D = 128 the difference between the instruction rate and
+// HBM as the bound.  q is scaled there by a power of two per head to fp16's upper range; a
+// value's scale v_scale goes into the exponent, w_j = exp2(s_j + log2 v_scale_j - max + 14), which fp16
+// holds whatever the scales.
 constexpr int kWarps = 4, kStep = 16, kTileKeys = kWarps * kStep;
 
 struct AttnArgs {
@@ -244,14 +253,17 @@ struct AttnArgs {
     int64_t q_stride;
     const int32_t *lens;
     int n_q_heads, group, n_groups, window, page_shift;   // group: query heads per K/V head
+    int whole_steps, dense_steps;                         // a page holds whole steps of 16 keys; their rows lie side by side
     float scale;                                          // times log2(e)
     __nv_bfloat16 *out;
     float *lse;
     unsigned *status;
     float *part_o;                                        // [2 * grid][8 NT][D]
     float2 *part_ml;                                      // [2 * grid][8 NT]
-    int2 *split;                                          // per unit: first part's CTA, parts (0: none)
+    int *arrived;                                         // [kJoinLevels][2 * grid], zero between calls
 };
+constexpr int kMaxCtasPerSm = 3, kMaxUnitHeads = 16, kMaxGroups = 8;
+constexpr int kJoinWays = 16, kJoinLevels = 3;            // 16^3 parts
 
 template <int D, bool I8, int NT>
 struct AttnShape {
@@ -260,14 +272,14 @@ struct AttnShape {
     static constexpr int kStages = kRows >= 8192 ? 3 : kRows >= 4096 ? 4 : 6;
     static constexpr int kStage = kRows + (I8 ? 128 : 0) + 16;           // + scales, + live mask
     static constexpr int kHeads = 8 * NT;
-    static constexpr int kJoinRow = 68;                                  // 64 components, padded
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kJoinCols = 32, kJoinRow = kJoinCols + 4;
     static constexpr int kJoin = kWarps * kHeads * kJoinRow * 4;
     static constexpr int kQRow = D + 8;
-    static constexpr int kQ = D == 256 && NT == 2 ? kHeads * kQRow * 2 : 0;  // q in shared memory, see below
-    static constexpr int kRing = kWarps * kStages * kStage;              // the join reuses it
-    static constexpr int kSmem = kRing + kQ;
-    static constexpr int kCtas = kSmem > 112 * 1024 ? 1 : kSmem > 74 * 1024 ? 2 : 3;
-    static_assert(kJoin <= kRing, "join");
+    static constexpr int kQ = kHeads * kQRow * 2 + kHeads * 4;           // q, and an int8 pool's factors
+    static constexpr bool kQInRegs = !(D == 256 && NT == 2);             // 64 registers of q beside 128 of o would spill
+    static constexpr int kSmem = kRing + kJoin + kQ;
+    static constexpr int kCtas = 3 * (kSmem + 1800) <= 228 * 1024 ? 3 : 2 * (kSmem + 1800) <= 228 * 1024 ? 2 : 1;
 };
 
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool live) {
@@ -296,143 +308,320 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// two of a word's int8 bytes (picked by `sel`) to bf16 pairs, exactly: with v's sign bit s and low
-// bits w, v = (128 + w) - (128 + 128 s), and 0x4300 | w, 0x4300 | 128 s are those bf16 numbers
-__device__ __forceinline__ uint32_t bf16x2_of_i8(uint32_t word, uint32_t sel) {
-    const uint32_t u = __byte_perm(word, 0x43434343u, sel);
-    const uint32_t lo = u & 0xff7fff7fu, hi = u & 0xff80ff80u;
-    __nv_bfloat162 a, b;
-    a = *reinterpret_cast<const __nv_bfloat162 *>(&lo);
-    b = *reinterpret_cast<const __nv_bfloat162 *>(&hi);
-    const __nv_bfloat162 d = __hsub2(a, b);
+__device__ __forceinline__ float log2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// bytes sel of a word of int8 + 128 (the word with its sign bits flipped) as an fp16 pair, exactly:
+// 0x6400 | u is 1024 + u
+__device__ __forceinline__ uint32_t f16x2_of_u8(uint32_t word, uint32_t sel) {
+    const uint32_t u = __byte_perm(word, 0x64646464u, sel), off = 0x64806480u;   // 1024 + 128
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&u), *reinterpret_cast<const __half2 *>(&off));
     return *reinterpret_cast<const uint32_t *>(&d);
 }
-// (x, y) as the bf16 pair nearest and the pair of what that leaves
-__device__ __forceinline__ void split_bf16x2(float x, float y, uint32_t &hi, uint32_t &lo) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    const __nv_bfloat162 r = __floats2bfloat162_rn(x - xdna::bf16lo(hi), y - xdna::bf16hi(hi));
-    lo = *reinterpret_cast<const uint32_t *>(&r);
+// (x, y) as the 16-bit pair nearest and the pair of what that leaves
+template <bool F16>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t &hi, uint32_t &lo) {
+    if constexpr (F16) {
+        const __half2 h = __floats2half2_rn(x, y);
+        const float2 f = __half22float2(h);
+        const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
+        hi = *reinterpret_cast<const uint32_t *>(&h);
+        lo = *reinterpret_cast<const uint32_t *>(&r);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        hi = *reinterpret_cast<const uint32_t *>(&h);
+        const __nv_bfloat162 r = __floats2bfloat162_rn(x - xdna::bf16lo(hi), y - xdna::bf16hi(hi));
+        lo = *reinterpret_cast<const uint32_t *>(&r);
+    }
 }
 
-// live keys of stream b: [first, first + count)
-__device__ __forceinline__ int2 live_keys(const AttnArgs &a, int b) {
-    const int n = min(max(0, a.lens[b]), a.table.width * a.pool.page_size);
-    const int first = a.window && n > a.window ? n - a.window : 0;
-    return make_int2(first, n - first);
+// live keys of a stream of n tokens: [x, y); tiles are laid from `first`: with whole steps to a page, from
+// the step that holds x, so that no step crosses a page
+struct Live {
+    int x, y, first, tiles;
+};
+__device__ __forceinline__ Live live_keys(const AttnArgs &a, int n) {
+    Live k;
+    k.y = min(max(0, n), a.table.width * a.pool.page_size);
+    k.x = a.window && k.y > a.window ? k.y - a.window : 0;
+    k.first = a.whole_steps ? k.x & -kStep : k.x;
+    k.tiles = (k.y - k.first + kTileKeys - 1) / kTileKeys;
+    return k;
 }
-__device__ __forceinline__ int tiles_of(int keys) { return (keys + kTileKeys - 1) / kTileKeys; }
 
-template <int D, bool I8, int NT>
+template <int D, bool I8, int NT, bool kSmall>
 __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_kernel(const AttnArgs a) {
     using S = AttnShape<D, I8, NT>;
-    constexpr int kChunks = S::kRowBytes / 16, kRowsPerCopy = 32 / kChunks < 1 ? 1 : 32 / kChunks;
-    constexpr int kMt = D / 16;
+    constexpr int kChunks = S::kRowBytes / 16, kRowsPerCopy = kChunks >= 32 ? 1 : 32 / kChunks, kCopies = kStep / kRowsPerCopy;
+    constexpr int kMt = D / 16, kElem = I8 ? 1 : 2;
+    constexpr float kLift = I8 ? 14.0f : 0.0f;            // weights reach up to 2^kLift
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int scan[kWarps], where[4];
     __shared__ float join_m[kWarps][S::kHeads], join_l[kWarps][S::kHeads];
+    __shared__ int last;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, j = lane % 4;
     unsigned char *ring = smem + warp * S::kStages * S::kStage;
     const uint32_t ring_u = xdna::smem_u32(ring);
-    float *join_o = reinterpret_cast<float *>(smem);
-    __nv_bfloat16 *q_s = reinterpret_cast<__nv_bfloat16 *>(smem + S::kRing);
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    float *join_o = reinterpret_cast<float *>(smem + S::kRing);
+    uint16_t *q_s = reinterpret_cast<uint16_t *>(smem + S::kRing + S::kJoin);
+    float *q_inv = reinterpret_cast<float *>(q_s + S::kHeads * S::kQRow);
+    // ---- streams of no keys, once the CTA is through
+    auto empty_streams = [&]() {
+        for (int b = blockIdx.x; b < a.table.n_seqs; b += gridDim.x) {
+            const int n = a.lens[b];
+            if (n > a.table.width * a.pool.page_size && tid == 0) atomicOr(a.status, kBadPosition);
+            if (n > 0) continue;
+            uint4 *out = reinterpret_cast<uint4 *>(a.out + (int64_t)b * a.n_q_heads * D);
+            for (int i = tid; i < a.n_q_heads * (D / 8); i += 128) out[i] = make_uint4(0, 0, 0, 0);
+            if (a.lse)
+                for (int i = tid; i < a.n_q_heads; i += 128) a.lse[(int64_t)b * a.n_q_heads + i] = -INFINITY;
+        }
+    };
 
-    // ---- this CTA's share: tiles [share0, share1) of all units laid end to end
+    // ---- this CTA's share: tiles [share0, share1) of all units laid end to end.  Every warp works it out
+    // for itself, 128 streams at a time, 4 to a lane.
     const int units_per_stream = a.pool.n_kv_heads * a.n_groups, B = a.table.n_seqs;
-    auto block_scan = [&](int x, int &total) {            // inclusive, over the 128 threads
+    int tiles4[4], mine = 0, upto = 0;                    // a lane's streams, their sum, the sum up to them
+    auto count128 = [&](int b0) {
+        mine = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int b = b0 + lane * 4 + k;
+            mine += tiles4[k] = b < B ? live_keys(a, a.lens[b]).tiles : 0;
+        }
+        upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
-            const int y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
         }
-        __syncthreads();
-        if (lane == 31) scan[warp] = x;
-        __syncthreads();
-        total = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-            if (w < warp) x += scan[w];
-            total += scan[w];
-        }
-        return x;
+        return __shfl_sync(0xffffffffu, upto, 31);
     };
-    int64_t total = 0;
-    int mine = 0, upto = 0;
-    for (int b0 = 0; b0 < B; b0 += 128) {
-        mine = b0 + tid < B ? tiles_of(live_keys(a, b0 + tid).y) : 0;
-        int sum;
-        upto = block_scan(mine, sum);
-        total += sum;
-    }
+    using Int = std::conditional_t<kSmall, int, int64_t>;  // total * ctas fits
+    Int total = 0;
+    for (int b0 = 0; b0 < B; b0 += 128) total += count128(b0);
     total *= units_per_stream;
+    if (total == 0) {
+        empty_streams();
+        return;
+    }
     // no share is empty, so that a unit's parts lie in consecutive CTAs
-    const int ctas = (int)min((int64_t)gridDim.x, total);
-    if ((int)blockIdx.x >= ctas) return;
-    const int64_t share0 = total * blockIdx.x / ctas, share1 = total * (blockIdx.x + 1) / ctas;
-    int64_t before = 0;                                   // tiles of one head of the streams before b0
+    const Int units = (Int)B * units_per_stream;
+    Int want = min((Int)gridDim.x, total);
+    if (total <= units * (4 * kJoinWays)) want = min(want, units * kJoinWays);
+    if (units < want && total < 8 * want) want = want / units * units;
+    const int ctas = (int)want;
+    if ((int)blockIdx.x >= ctas) {
+        empty_streams();
+        return;
+    }
+    const Int share0 = total * (Int)blockIdx.x / ctas, share1 = total * (Int)(blockIdx.x + 1) / ctas;
+    int at_b = 0, at_unit = 0, at_tile = 0;
+    Int before = 0;                                       // tiles of one head of the streams before b0
     for (int b0 = 0; b0 < B; b0 += 128) {
-        int sum;
-        if (B > 128) {
-            mine = b0 + tid < B ? tiles_of(live_keys(a, b0 + tid).y) : 0;
-            upto = block_scan(mine, sum);
-        } else {
-            sum = 0x7fffffff;
-        }
-        if ((before + sum) * units_per_stream > share0) {
-            const int64_t from = (before + upto - mine) * units_per_stream;
-            if (mine && from <= share0 && share0 < from + (int64_t)mine * units_per_stream) {
-                where[0] = b0 + tid;
-                where[1] = (int)((share0 - from) / mine);
-                where[2] = (int)((share0 - from) % mine);
+        const int sum = B > 128 ? count128(b0) : 0;
+        if (B <= 128 || (before + sum) * units_per_stream > share0) {
+            Int from = (before + upto - mine) * units_per_stream;
+            const bool here = mine && from <= share0 && share0 < from + (Int)mine * units_per_stream;
+            int k = 0, n = max(1, tiles4[0]);
+#pragma unroll
+            for (int q = 0; q < 3; q++) {
+                const Int next = from + (Int)tiles4[q] * units_per_stream;
+                if (k == q && share0 >= next) {
+                    from = next;
+                    k = q + 1;
+                    n = max(1, tiles4[q + 1]);
+                }
             }
+            const Int off = here ? share0 - from : 0;
+            const int unit = (int)(off / n), tile = (int)(off - (Int)unit * n);
+            const int owner = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+            at_b = __shfl_sync(0xffffffffu, b0 + lane * 4 + k, owner);
+            at_unit = __shfl_sync(0xffffffffu, unit, owner);
+            at_tile = __shfl_sync(0xffffffffu, tile, owner);
             break;
         }
         before += sum;
     }
-    __syncthreads();
-    int b = where[0], unit = where[1], t0 = where[2];
-    int2 live = live_keys(a, b);
-    int tiles = tiles_of(live.y);
-    if (tid == 0 && a.lens[b] > a.table.width * a.pool.page_size) atomicOr(a.status, kBadPosition);
 
-    for (int64_t at = share0; at < share1;) {
-        const int t1 = (int)min((int64_t)tiles, t0 + (share1 - at));
-        const int hk = unit / a.n_groups, h0 = hk * a.group + (unit % a.n_groups) * S::kHeads;
-        const int heads = min(S::kHeads, a.group - (unit % a.n_groups) * S::kHeads);
-        const unsigned char *kb = static_cast<const unsigned char *>(a.pool.k) + hk * a.pool.sh * (I8 ? 1 : 2);
-        const unsigned char *vb = static_cast<const unsigned char *>(a.pool.v) + hk * a.pool.sh * (I8 ? 1 : 2);
-        const int32_t *ids = a.table.ids + b * a.table.stride;
-        const int end = live.x + live.y;
+    // ---- a place in the share: a unit of a stream, and a tile of its keys
+    struct Place {
+        int b, unit, t;
+        Live live;
+    };
+    auto next_unit = [&](Place &p) {                      // only within the share: there is one
+        p.t = 0;
+        if (++p.unit == units_per_stream) {
+            p.unit = 0;
+            do {
+                if (++p.b >= B) { p.b = B - 1; return; }
+                p.live = live_keys(a, a.lens[p.b]);
+            } while (p.live.tiles == 0);
+        }
+    };
+    Place at{at_b, at_unit, at_tile, live_keys(a, a.lens[at_b])}, ahead = at;
+    int left = (int)(share1 - share0), unfetched = left;
 
-        // ---- q of the unit's heads as the products' 8-column operand: pair (2j, 2j + 1) and (2j + 8,
-        // 2j + 9) of each 16 components; an int8 row's words hold 4 components in order, so there the
-        // pairs are (4j, 4j + 1) and (4j + 2, 4j + 3), in K and q alike
-        uint32_t qf[S::kQ ? 1 : NT][S::kQ ? 1 : kMt][2];
-        const __nv_bfloat16 *q = a.q + b * a.q_stride + (int64_t)h0 * D;
-        if constexpr (S::kQ) {                            // 64 registers of q beside 128 of o would spill
-            __syncthreads();
-            for (int i = tid; i < S::kHeads * D / 2; i += 128)
-                reinterpret_cast<uint32_t *>(q_s)[i / (D / 2) * (S::kQRow / 2) + i % (D / 2)] =
-                    i / (D / 2) < heads ? reinterpret_cast<const uint32_t *>(q)[i] : 0u;
-            __syncthreads();
-        } else {
+    // ---- the ring.  issue() copies the step of the place `ahead`, whose page (that of its key r in lanes r
+    // and r + 16, where steps do not lie whole in pages) look_up() fetched a step before, and moves on.
+    int ahead_hk = ahead.unit / a.n_groups;
+    auto look_up = [&](int t, int row) {
+        const int key = ahead.live.first + (t * kWarps + warp) * kStep + row;
+        return t < ahead.live.tiles && key < ahead.live.y
+                   ? a.table.ids[ahead.b * a.table.stride + (a.page_shift >= 0 ? key >> a.page_shift : key / a.pool.page_size)]
+                   : -1;
+    };
+    const int own_row = a.whole_steps ? 0 : lane & 15;
+    const int lane_row = lane / kChunks, lane_chunk = lane % kChunks;
+    auto swizzled = [](int r, int chunk) { return r * S::kRowBytes + ((chunk ^ (kChunks >= 8 ? r & 7 : (r >> 1) & 3)) * 16); };
+    const int64_t kv = static_cast<const unsigned char *>(a.pool.v) - static_cast<const unsigned char *>(a.pool.k);
+    auto issue = [&](int stage, int page) {
+        if (unfetched <= 0) return;
+        const uint32_t base = ring_u + stage * S::kStage;
+        const int pos = ahead.live.first + (ahead.t * kWarps + warp) * kStep;
+        const unsigned char *kb = static_cast<const unsigned char *>(a.pool.k) + ahead_hk * a.pool.sh * kElem;
+        unsigned mask = 0xffffu;
+        if (a.dense_steps && pos >= ahead.live.x && pos + kStep <= ahead.live.y && (unsigned)page < (unsigned)a.pool.n_pages) {
+            // 16 whole rows side by side
+            const int slot = a.page_shift >= 0 ? pos & ((1 << a.page_shift) - 1) : pos % a.pool.page_size;
+            const unsigned char *at = kb + page * a.pool.sp * kElem + slot * S::kRowBytes + lane * 16;
+#pragma unroll
+            for (int i = 0; i < kCopies; i++) {
+                const uint32_t dst = base + swizzled(i * kRowsPerCopy + lane_row, lane_chunk);
+                cp_async16_or_zero(dst, at + i * 512, true);
+                cp_async16_or_zero(dst + kStep * S::kRowBytes, at + kv + i * 512, true);
+            }
+            if constexpr (I8) {                           // lanes 0-15 the keys' scales, 16-31 the values'
+                const int64_t r = ((int64_t)page * a.pool.n_kv_heads + ahead_hk) * a.pool.page_size + slot + (lane & 15);
+                cp_async4_or_zero(base + S::kRows + lane * 4, (lane < 16 ? a.pool.ks : a.pool.vs) + r, true);
+            }
+        } else {                                          // row by row: lane r looks after row r
+            const int row = lane & 15, key = pos + row, from = a.whole_steps ? pos : key;
+            const int slot = (a.page_shift >= 0 ? from & ((1 << a.page_shift) - 1) : from % a.pool.page_size) + key - from;
+            bool ok = key >= ahead.live.x && key < ahead.live.y;
+            if (ok && (unsigned)page >= (unsigned)a.pool.n_pages) {
+                atomicOr(a.status, kBadPage);
+                ok = false;
+            }
+            mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+            const int64_t off = ok ? page * a.pool.sp * kElem + slot * a.pool.ss * kElem : -1;
+#pragma unroll 1
+            for (int r = lane_row; r < kStep; r += kRowsPerCopy) {
+                const int64_t at = __shfl_sync(0xffffffffu, off, r);
+                const unsigned char *src = kb + (at < 0 ? 0 : at + lane_chunk * 16);
+                const uint32_t dst = base + swizzled(r, lane_chunk);
+                cp_async16_or_zero(dst, src, at >= 0);
+                cp_async16_or_zero(dst + kStep * S::kRowBytes, src + kv, at >= 0);
+            }
+            if constexpr (I8) {
+                const int64_t r = ok ? ((int64_t)page * a.pool.n_kv_heads + ahead_hk) * a.pool.page_size + slot : 0;
+                cp_async4_or_zero(base + S::kRows + lane * 4, (lane < 16 ? a.pool.ks : a.pool.vs) + r, ok);
+            }
+        }
+        if (lane == 0) *reinterpret_cast<unsigned *>(ring + stage * S::kStage + S::kStage - 16) = mask;
+        if (--unfetched == 0) return;
+        if (++ahead.t == ahead.live.tiles) {
+            next_unit(ahead);
+            ahead_hk = ahead.unit / a.n_groups;
+        }
+    };
+
+    // ---- q: warp w takes heads w, w + 4, ..., a lane D / 32 components, from global memory to registers
+    // (load_q), to 16 bits in shared memory (store_q), from there as the products' 8-column operand:
+    // pair (2j, 2j + 1) and (2j + 8, 2j + 9) of each 16 components; an int8 row's words hold 4 components
+    // in order, so there the pairs are (4j, 4j + 1) and (4j + 2, 4j + 3), in K and q alike
+    constexpr int kQWords = D / 64;
+    uint32_t q_in[S::kHeads / kWarps][kQWords];
+    uint32_t qf[S::kQInRegs ? NT : 1][S::kQInRegs ? kMt : 1][2];
+    auto load_q = [&](const Place &p) {
+        const int first = p.unit % a.n_groups * S::kHeads;
+        const __nv_bfloat16 *q = a.q + p.b * a.q_stride + (int64_t)(p.unit / a.n_groups * a.group + first) * D;
+#pragma unroll
+        for (int i = 0; i < S::kHeads / kWarps; i++)
+#pragma unroll
+            for (int w = 0; w < kQWords; w++)
+                q_in[i][w] = first + warp + kWarps * i < a.group
+                                 ? reinterpret_cast<const uint32_t *>(q + (warp + kWarps * i) * D)[lane * kQWords + w]
+                                 : 0u;
+    };
+    auto store_q = [&]() {
+#pragma unroll
+        for (int i = 0; i < S::kHeads / kWarps; i++) {
+            const int h = warp + kWarps * i;
+            if constexpr (I8) {
+                float top = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kQWords; w++)
+                    top = fmaxf(top, fmaxf(fabsf(xdna::bf16lo(q_in[i][w])), fabsf(xdna::bf16hi(q_in[i][w]))));
+#pragma unroll
+                for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                // the largest to [2^13, 2^14), as far as the factor's own exponent reaches
+                const int e = max(1, min(253, 267 - (__float_as_int(top) >> 23)));
+                const float f = __int_as_float(e << 23);
+                if (lane == 0) q_inv[h] = __int_as_float((254 - e) << 23);
+#pragma unroll
+                for (int w = 0; w < kQWords; w++) {
+                    const __half2 v = __floats2half2_rn(xdna::bf16lo(q_in[i][w]) * f, xdna::bf16hi(q_in[i][w]) * f);
+                    q_in[i][w] = *reinterpret_cast<const uint32_t *>(&v);
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < kQWords; w++)
+                reinterpret_cast<uint32_t *>(q_s + h * S::kQRow)[lane * kQWords + w] = q_in[i][w];
+        }
+    };
+    auto q_word = [&](int nt, int c, int i) -> uint32_t {
+        return *reinterpret_cast<const uint32_t *>(q_s + (nt * 8 + g) * S::kQRow + 16 * c + (I8 ? 4 * j + 2 * i : 2 * j + 8 * i));
+    };
+    float q_back[NT][2];                                  // an int8 pool's factors of heads 2j, 2j + 1
+    auto take_q = [&]() {
+        if constexpr (S::kQInRegs) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int c = 0; c < kMt; c++) {
-                    const int h = nt * 8 + g, e0 = 16 * c + (I8 ? 4 * j : 2 * j), e1 = e0 + (I8 ? 2 : 8);
-                    qf[nt][c][0] = h < heads ? *reinterpret_cast<const uint32_t *>(q + h * D + e0) : 0u;
-                    qf[nt][c][1] = h < heads ? *reinterpret_cast<const uint32_t *>(q + h * D + e1) : 0u;
+                    qf[nt][c][0] = q_word(nt, c, 0);
+                    qf[nt][c][1] = q_word(nt, c, 1);
                 }
         }
+        if constexpr (I8) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) q_back[nt][i] = q_inv[nt * 8 + 2 * j + i] * a.scale;
+        }
+    };
+    load_q(at);
+    const int same_unit = a.whole_steps ? min(32, ahead.live.tiles - ahead.t) : 0;
+    const int first_pages = look_up(ahead.t + lane, 0);   // lane i: the first unit's step i
+#pragma unroll 1
+    for (int i = 0; i < S::kStages - 1; i++) {
+        const int page = __shfl_sync(0xffffffffu, first_pages, i);
+        issue(i, i < same_unit ? page : look_up(ahead.t, own_row));
+        xdna::cp_async_commit();
+    }
+    int page = look_up(ahead.t, own_row);
+    store_q();
+    __syncthreads();
+    take_q();
 
-        float o[NT][kMt][4], m[NT][2], ms[NT][2], l[NT][2];   // ms: m, or 0 while there is no maximum
+    int stage = 0;
+    for (;;) {
+        const int run = min(at.live.tiles - at.t, left);  // tiles of this unit
+        float o[NT][kMt][4], m[NT][2], ms[NT][2], l[NT][2];   // ms: m - kLift, or 0 while there is no maximum
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -442,57 +631,12 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
 #pragma unroll
             for (int i = 0; i < 2; i++) m[nt][i] = -INFINITY, ms[nt][i] = l[nt][i] = 0.0f;
         }
-
-        // ---- the ring: lane r (and r + 16) looks up key r's page a step ahead of its copy
-        auto key_of = [&](int t) { return live.x + (t * kWarps + warp) * kStep + (lane & 15); };
-        auto page_of = [&](int t) {
-            const int pos = key_of(t);
-            if (t >= t1 || pos >= end) return -1;
-            return ids[a.page_shift >= 0 ? pos >> a.page_shift : pos / a.pool.page_size];
-        };
-        auto issue = [&](int stage, int t, int page) {
-            const int pos = key_of(t);
-            bool ok = t < t1 && pos < end;
-            if (ok && (unsigned)page >= (unsigned)a.pool.n_pages) {
-                atomicOr(a.status, kBadPage);
-                ok = false;
-            }
-            const int slot = a.page_shift >= 0 ? pos & ((1 << a.page_shift) - 1) : pos % a.pool.page_size;
-            const int64_t row = ok ? (page * a.pool.sp + slot * a.pool.ss) * (I8 ? 1 : 2) : -1;
-            const unsigned mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-            const uint32_t base = ring_u + stage * S::kStage;
-            if (lane == 0) *reinterpret_cast<unsigned *>(ring + stage * S::kStage + S::kStage - 16) = mask;
-#pragma unroll
-            for (int i = 0; i < kStep / kRowsPerCopy; i++) {
-                const int r = i * kRowsPerCopy + (kChunks < 32 ? lane / kChunks : 0), c = lane % kChunks;
-                const int64_t off = __shfl_sync(0xffffffffu, row, r);
-                const uint32_t dst = base + r * S::kRowBytes + ((c ^ (kChunks >= 8 ? r & 7 : (r >> 1) & 3)) * 16);
-                const int64_t from = off < 0 ? 0 : off + c * 16;
-                cp_async16_or_zero(dst, kb + from, off >= 0);
-                cp_async16_or_zero(dst + kStep * S::kRowBytes, vb + from, off >= 0);
-            }
-            if constexpr (I8) {
-                const int64_t r = ok ? ((int64_t)page * a.pool.n_kv_heads + hk) * a.pool.page_size + slot : 0;
-                cp_async4_or_zero(base + S::kRows + lane * 4, (lane < 16 ? a.pool.ks : a.pool.vs) + r, ok);
-            }
-        };
-        int page = page_of(t0);
-#pragma unroll
-        for (int i = 0; i < S::kStages - 1; i++) {
-            const int next = page_of(t0 + i + 1);
-            if (t0 + i < t1) issue(i, t0 + i, page);
-            xdna::cp_async_commit();
-            page = next;
-        }
-        int stage = 0;
-        for (int t = t0; t < t1; t++) {
+        for (int t = 0; t < run; t++) {
             xdna::cp_async_wait_group<S::kStages - 2>();
             __syncwarp();
-            const int last = stage == 0 ? S::kStages - 1 : stage - 1;
-            const int next = page_of(t + S::kStages);
-            if (t + S::kStages - 1 < t1) issue(last, t + S::kStages - 1, page);
+            issue(stage == 0 ? S::kStages - 1 : stage - 1, page);
             xdna::cp_async_commit();
-            page = next;
+            page = look_up(ahead.t, own_row);
 
             const uint32_t ks = ring_u + stage * S::kStage, vs = ks + kStep * S::kRowBytes;
             const unsigned char *tail = ring + stage * S::kStage + S::kRows;
@@ -506,11 +650,8 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
                     for (int i = 0; i < 4; i++) s[nt][0][i] = s[nt][1][i] = 0.0f;
                 const int r = lane & 15, sw = kChunks >= 8 ? r & 7 : (r >> 1) & 3;
                 auto q_of = [&](int nt, int c, int i) -> uint32_t {
-                    if constexpr (S::kQ)
-                        return *reinterpret_cast<const uint32_t *>(
-                            q_s + (nt * 8 + g) * S::kQRow + 16 * c + (I8 ? 4 * j + 2 * i : 2 * j + 8 * i));
-                    else
-                        return qf[nt][c][i];
+                    if constexpr (S::kQInRegs) return qf[nt][c][i];
+                    else return q_word(nt, c, i);
                 };
                 if constexpr (!I8) {
 #pragma unroll
@@ -527,31 +668,38 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
                         uint32_t k[4];
                         ldsm4(k, ks + r * S::kRowBytes + (((c + (lane >> 4)) ^ sw) * 16));
 #pragma unroll
+                        for (int x = 0; x < 4; x++) k[x] ^= 0x80808080u;
+#pragma unroll
                         for (int x = 0; x < 2; x++) {
-                            const uint32_t a0 = bf16x2_of_i8(k[2 * x], 0x4140), a2 = bf16x2_of_i8(k[2 * x], 0x4342);
-                            const uint32_t a1 = bf16x2_of_i8(k[2 * x + 1], 0x4140), a3 = bf16x2_of_i8(k[2 * x + 1], 0x4342);
+                            const uint32_t a0 = f16x2_of_u8(k[2 * x], 0x4140), a2 = f16x2_of_u8(k[2 * x], 0x4342);
+                            const uint32_t a1 = f16x2_of_u8(k[2 * x + 1], 0x4140), a3 = f16x2_of_u8(k[2 * x + 1], 0x4342);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++)
-                                mma_bf16(s[nt][x], a0, a1, a2, a3, q_of(nt, c + x, 0), q_of(nt, c + x, 1));
+                                mma_f16(s[nt][x], a0, a1, a2, a3, q_of(nt, c + x, 0), q_of(nt, c + x, 1));
                         }
                     }
                 }
                 // ---- running maximum and weights
                 const bool ok0 = (mask >> g) & 1, ok1 = (mask >> (g + 8)) & 1;
-                float f0 = a.scale, f1 = a.scale, v0 = 1.0f, v1 = 1.0f;
+                float f0 = a.scale, f1 = a.scale, v0 = 0.0f, v1 = 0.0f;
                 if constexpr (I8) {
                     const float *sc = reinterpret_cast<const float *>(tail);
-                    f0 *= sc[g]; f1 *= sc[g + 8];
-                    v0 = sc[16 + g]; v1 = sc[24 + g];
+                    f0 = sc[g]; f1 = sc[g + 8];
+                    v0 = log2_approx(fmaxf(sc[16 + g], 1e-30f));
+                    v1 = log2_approx(fmaxf(sc[24 + g], 1e-30f));
                 }
+                float den[NT][4];                         // the exponents of the sum's terms, s[.][0] the weights'
                 bool up = false;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        s[nt][0][i] = ok0 ? (s[nt][0][i] + s[nt][1][i]) * f0 : -INFINITY;
-                        s[nt][0][2 + i] = ok1 ? (s[nt][0][2 + i] + s[nt][1][2 + i]) * f1 : -INFINITY;
-                        up |= fmaxf(s[nt][0][i], s[nt][0][2 + i]) > m[nt][i];
+                    for (int i = 0; i < 4; i++) {
+                        float x = (s[nt][0][i] + s[nt][1][i]) * (i < 2 ? f0 : f1);
+                        if constexpr (I8) x *= q_back[nt][i & 1];
+                        x = (i < 2 ? ok0 : ok1) ? x : -INFINITY;
+                        den[nt][i] = x;
+                        s[nt][0][i] = I8 ? x + (i < 2 ? v0 : v1) : x;
+                        up |= s[nt][0][i] > m[nt][i & 1];
                     }
                 if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -564,7 +712,7 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
                             for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                             corr[i] = top == m[nt][i] ? 1.0f : exp2_approx(m[nt][i] - top);
                             m[nt][i] = top;
-                            ms[nt][i] = top == -INFINITY ? 0.0f : top;
+                            ms[nt][i] = top == -INFINITY ? 0.0f : top - kLift;
                             l[nt][i] *= corr[i];
                         }
 #pragma unroll
@@ -581,11 +729,10 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         p[i] = exp2_approx(s[nt][0][i] - ms[nt][i & 1]);
-                        l[nt][i & 1] += p[i];
-                        if constexpr (I8) p[i] *= i < 2 ? v0 : v1;
+                        l[nt][i & 1] += I8 ? exp2_approx(den[nt][i] - ms[nt][i & 1]) : p[i];
                     }
-                    split_bf16x2(p[0], p[1], ph[nt][0], pl[nt][0]);
-                    split_bf16x2(p[2], p[3], ph[nt][1], pl[nt][1]);
+                    split_pair<I8>(p[0], p[1], ph[nt][0], pl[nt][0]);
+                    split_pair<I8>(p[2], p[3], ph[nt][1], pl[nt][1]);
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         ph[nt][i] = transpose8x8(ph[nt][i]);
@@ -612,13 +759,15 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
                         uint32_t v[4];
                         ldsm4_trans(v, vs + r * S::kRowBytes + (((c + (lane >> 4)) ^ sw) * 16));
 #pragma unroll
+                        for (int x = 0; x < 4; x++) v[x] ^= 0x80808080u;
+#pragma unroll
                         for (int x = 0; x < 2; x++) {
-                            const uint32_t a0 = bf16x2_of_i8(v[2 * x], 0x4240), a1 = bf16x2_of_i8(v[2 * x], 0x4341);
-                            const uint32_t a2 = bf16x2_of_i8(v[2 * x + 1], 0x4240), a3 = bf16x2_of_i8(v[2 * x + 1], 0x4341);
+                            const uint32_t a0 = f16x2_of_u8(v[2 * x], 0x4240), a1 = f16x2_of_u8(v[2 * x], 0x4341);
+                            const uint32_t a2 = f16x2_of_u8(v[2 * x + 1], 0x4240), a3 = f16x2_of_u8(v[2 * x + 1], 0x4341);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
-                                mma_bf16(o[nt][c + x], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-                                mma_bf16(o[nt][c + x], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+                                mma_f16(o[nt][c + x], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+                                mma_f16(o[nt][c + x], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
                             }
                         }
                     }
@@ -627,21 +776,33 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
             __syncwarp();
             stage = stage + 1 == S::kStages ? 0 : stage + 1;
         }
-        xdna::cp_async_wait_all();
 
-        // ---- the warps' parts into one
+        // ---- the unit's end: the warps' parts into one, the next unit's q on its way meanwhile
+        const Place done = at;
+        left -= run;
+        if (left) {
+            next_unit(at);
+            load_q(at);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
 #pragma unroll
                 for (int x = 4; x < 32; x *= 2) l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], x);
+                m[nt][i] -= kLift;
                 if (g == 0) {
                     join_m[warp][nt * 8 + 2 * j + i] = m[nt][i];
                     join_l[warp][nt * 8 + 2 * j + i] = l[nt][i];
                 }
             }
+        if (!left) xdna::cp_async_wait_all();
         __syncthreads();
+        if (left) store_q();
+        const int hk = done.unit / a.n_groups, h0 = hk * a.group + (done.unit % a.n_groups) * S::kHeads;
+        const int heads = min(S::kHeads, a.group - (done.unit % a.n_groups) * S::kHeads);
+        const bool whole = done.t == 0 && run == done.live.tiles;
+        const int slot = 2 * blockIdx.x + (done.t == 0);
         float fac[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -653,157 +814,172 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
                 for (int w = 1; w < kWarps; w++) top = fmaxf(top, join_m[w][h]);
                 fac[nt][i] = m[nt][i] == top ? 1.0f : exp2_approx(m[nt][i] - top);
             }
-        const bool whole = t0 == 0 && t1 == tiles;
-        const int slot = 2 * blockIdx.x + (t0 == 0);
+        auto of_warps = [&](int h, float &top, float &den) {
+            top = join_m[0][h];
+            den = 0.0f;
 #pragma unroll
-        for (int d0 = 0; d0 < D; d0 += 64) {
-            if (d0) __syncthreads();
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int comp = 16 * c + (I8 ? 2 * g + (i >> 1) : g + 8 * (i >> 1));
-                        join_o[(warp * S::kHeads + nt * 8 + 2 * j + (i & 1)) * S::kJoinRow + comp] =
-                            o[nt][d0 / 16 + c][i] * fac[nt][i & 1];
-                    }
-            __syncthreads();
-            for (int x = tid; x < heads * 16; x += 128) {
-                const int h = x / 16, c = x % 16 * 4;
-                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int w = 0; w < kWarps; w++) {
-                    const float4 y = *reinterpret_cast<const float4 *>(&join_o[(w * S::kHeads + h) * S::kJoinRow + c]);
-                    sum.x += y.x; sum.y += y.y; sum.z += y.z; sum.w += y.w;
-                }
-                if (whole) {
-                    float top = join_m[0][h], den = 0.0f;
-#pragma unroll
-                    for (int w = 1; w < kWarps; w++) top = fmaxf(top, join_m[w][h]);
-#pragma unroll
-                    for (int w = 0; w < kWarps; w++)
-                        den += join_l[w][h] * (join_m[w][h] == top ? 1.0f : exp2_approx(join_m[w][h] - top));
-                    const float inv = 1.0f / den;
-                    const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * inv, sum.y * inv),
-                                         hi = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
-                    *reinterpret_cast<uint2 *>(a.out + ((int64_t)b * a.n_q_heads + h0 + h) * D + d0 + c) =
-                        make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-                } else {
-                    *reinterpret_cast<float4 *>(a.part_o + ((int64_t)slot * S::kHeads + h) * D + d0 + c) = sum;
-                }
-            }
-        }
-        if (tid < heads) {
-            float top = join_m[0][tid], den = 0.0f;
-#pragma unroll
-            for (int w = 1; w < kWarps; w++) top = fmaxf(top, join_m[w][tid]);
+            for (int w = 1; w < kWarps; w++) top = fmaxf(top, join_m[w][h]);
 #pragma unroll
             for (int w = 0; w < kWarps; w++)
-                den += join_l[w][tid] * (join_m[w][tid] == top ? 1.0f : exp2_approx(join_m[w][tid] - top));
-            if (!whole) a.part_ml[slot * S::kHeads + tid] = make_float2(top, den);
-            else if (a.lse) a.lse[(int64_t)b * a.n_q_heads + h0 + tid] = (top + log2f(den)) * 0.69314718f;
+                den += join_l[w][h] * (join_m[w][h] == top ? 1.0f : exp2_approx(join_m[w][h] - top));
+        };
+        auto join_warps = [&](auto columns) {             // that many components at a time
+            constexpr int kCols = decltype(columns)::value, kRow = kCols + 4;
+#pragma unroll
+            for (int d0 = 0; d0 < D; d0 += kCols) {
+                if (d0) __syncthreads();
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int c = 0; c < kCols / 16; c++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int comp = 16 * c + (I8 ? 2 * g + (i >> 1) : g + 8 * (i >> 1));
+                            join_o[(warp * S::kHeads + nt * 8 + 2 * j + (i & 1)) * kRow + comp] =
+                                o[nt][d0 / 16 + c][i] * fac[nt][i & 1];
+                        }
+                __syncthreads();
+                for (int x = tid; x < heads * (kCols / 4); x += 128) {
+                    const int h = x / (kCols / 4), c = x % (kCols / 4) * 4;
+                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int w = 0; w < kWarps; w++) {
+                        const float4 y = *reinterpret_cast<const float4 *>(&join_o[(w * S::kHeads + h) * kRow + c]);
+                        sum.x += y.x; sum.y += y.y; sum.z += y.z; sum.w += y.w;
+                    }
+                    if (whole) {
+                        float top, den;
+                        of_warps(h, top, den);
+                        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+                        const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * inv, sum.y * inv),
+                                             hi = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
+                        *reinterpret_cast<uint2 *>(a.out + ((int64_t)done.b * a.n_q_heads + h0 + h) * D + d0 + c) =
+                            make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+                    } else {
+                        *reinterpret_cast<float4 *>(a.part_o + ((int64_t)slot * S::kHeads + h) * D + d0 + c) = sum;
+                    }
+                }
+            }
+        };
+        if (left) {
+            join_warps(std::integral_constant<int, S::kJoinCols>{});
+        } else {                                          // the ring is free: all at once
+            join_o = reinterpret_cast<float *>(smem);
+            join_warps(std::integral_constant<int, D>{});
         }
-        if (t0 == 0 && tid == 0) {                        // which CTAs hold the unit's parts
-            int2 *sp = a.split + (int64_t)b * units_per_stream + unit;
-            if (whole) {
-                *sp = make_int2(0, 0);
-            } else {
-                const int64_t stop = at + tiles - 1;      // the unit's last tile lies in share `to`
-                const int64_t to = ((stop + 1) * ctas - 1) / total;
-                *sp = make_int2(blockIdx.x, (int)to - (int)blockIdx.x + 1);
+        if (tid < heads) {
+            float top, den;
+            of_warps(tid, top, den);
+            if (!whole) a.part_ml[slot * S::kHeads + tid] = make_float2(top, den);
+            else if (a.lse) a.lse[(int64_t)done.b * a.n_q_heads + h0 + tid] = (top + log2f(den)) * 0.69314718f;
+        }
+        if (!whole) {
+            // ---- parts: a unit's tiles [begin, begin + tiles) lie in the shares of CTAs first .. first + parts - 1
+            __threadfence();
+            __syncthreads();
+            const Int begin = share1 - left - run - done.t;
+            const int first = (int)(((begin + 1) * ctas - 1) / total);
+            const int parts = (int)(((begin + done.live.tiles) * ctas - 1) / total) - first + 1;
+            for (int level = 0, n = parts, i = blockIdx.x - first, stride = 1; level < kJoinLevels; level++) {
+                const int group = i / kJoinWays, size = min(kJoinWays, n - group * kJoinWays);
+                auto slot_of = [&](int k) {                   // a CTA's first unit is in its slot 0, unless it begins there
+                    const int part = (group * kJoinWays + k) * stride;
+                    return 2 * (first + part) + (part == 0);
+                };
+                if (size > 1) {
+                    if (tid == 0) {
+                        int *count = a.arrived + level * 2 * gridDim.x + slot_of(0);
+                        last = atomicAdd(count, 1) == size - 1;
+                        if (last) *count = 0;
+                    }
+                    __syncthreads();
+                    if (!last) break;
+                    __threadfence();
+                    const bool final = n <= kJoinWays;
+                    // 128 / heads threads a head: the weights once, then their columns
+                    const int per_head = 128 / heads, h = tid / per_head;
+                    if (h < heads) {
+                        const int64_t hop = (int64_t)2 * stride * S::kHeads;    // from part to part, in rows
+                        const int64_t row0 = (int64_t)slot_of(0) * S::kHeads + h, row1 = (int64_t)slot_of(1) * S::kHeads + h - hop;
+                        float2 ml[kJoinWays];
+                        constexpr int kUnder = S::kCtas < 3 && NT == 1 ? 16 : 8;   // loads under way, as registers allow
+                        float4 y[kUnder];
+                        auto load = [&](int k0, int c) {
+#pragma unroll
+                            for (int k = 0; k < kUnder; k++)
+                                y[k] = k0 + k < size ? __ldcg(reinterpret_cast<const float4 *>(
+                                                           a.part_o + (k0 + k ? row1 + (k0 + k) * hop : row0) * D + c))
+                                                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        };
+#pragma unroll
+                        for (int k = 0; k < kJoinWays; k++)
+                            ml[k] = k < size ? __ldcg(a.part_ml + (k ? row1 + k * hop : row0)) : make_float2(-INFINITY, 0.0f);
+                        int c = tid % per_head * 4;
+                        if (c < D) load(0, c);
+                        float top = ml[0].x, den = 0.0f;
+#pragma unroll
+                        for (int k = 1; k < kJoinWays; k++) top = fmaxf(top, ml[k].x);
+#pragma unroll
+                        for (int k = 0; k < kJoinWays; k++) {
+                            ml[k].x = ml[k].x == top ? 1.0f : exp2_approx(ml[k].x - top);
+                            if (k < size) den = fmaf(ml[k].y, ml[k].x, den);
+                        }
+                        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+#pragma unroll 1
+                        for (; c < D; c += per_head * 4) {
+                            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                            for (int k = 0; k < kJoinWays; k++) {
+                                if (k == kUnder) {
+                                    if (size <= kUnder) break;
+                                    load(kUnder, c);
+                                }
+                                if (k < size) {
+                                    sum.x = fmaf(y[k % kUnder].x, ml[k].x, sum.x); sum.y = fmaf(y[k % kUnder].y, ml[k].x, sum.y);
+                                    sum.z = fmaf(y[k % kUnder].z, ml[k].x, sum.z); sum.w = fmaf(y[k % kUnder].w, ml[k].x, sum.w);
+                                }
+                            }
+                            if (final) {
+                                const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * inv, sum.y * inv),
+                                                     hi = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
+                                *reinterpret_cast<uint2 *>(a.out + ((int64_t)done.b * a.n_q_heads + h0 + h) * D + c) = make_uint2(
+                                    *reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+                            } else {                          // in place of the group's first part: this thread alone reads it
+                                *reinterpret_cast<float4 *>(a.part_o + row0 * D + c) = sum;
+                            }
+                            if (c + per_head * 4 < D) load(0, c + per_head * 4);
+                        }
+                        if (tid % per_head == 0) {
+                            if (!final) join_m[0][h] = top, join_l[0][h] = den;
+                            else if (a.lse) a.lse[(int64_t)done.b * a.n_q_heads + h0 + h] = (top + log2f(den)) * 0.69314718f;
+                        }
+                    }
+                    if (final) break;
+                    __syncthreads();
+                    // the new maximum and sum after all threads have read the old
+                    if (tid < heads) a.part_ml[slot_of(0) * S::kHeads + tid] = make_float2(join_m[0][tid], join_l[0][tid]);
+                    __threadfence();
+                    __syncthreads();
+                }
+                i = group;
+                n = (n + kJoinWays - 1) / kJoinWays;
+                stride *= kJoinWays;
             }
         }
+        if (!left) break;
         __syncthreads();
-        at += t1 - t0;
-        t0 = 0;
-        if (at < share1 && ++unit == units_per_stream) {
-            unit = 0;
-            do {
-                if (++b == B) return;
-                live = live_keys(a, b);
-            } while (live.y == 0);
-            tiles = tiles_of(live.y);
-            if (tid == 0 && a.lens[b] > a.table.width * a.pool.page_size) atomicOr(a.status, kBadPosition);
-        }
+        take_q();
     }
-}
 
-// One CTA per unit and head: a stream of no keys gets zeros; a unit cut among CTAs gets the sum of its
-// parts, taken at the largest of their maxima, in CTA order.
-template <int D>
-__global__ void __launch_bounds__(256) join_kernel(const AttnArgs a, int unit_heads) {
-    constexpr int kCols = D / 4, kRowsAtOnce = 256 / kCols;
-    __shared__ float red[8], dens[8], weight[1024];
-    __shared__ float4 sums[256];
-    const int units = a.pool.n_kv_heads * a.n_groups, b = blockIdx.x / units, unit = blockIdx.x % units;
-    const int first = (unit % a.n_groups) * unit_heads, h = blockIdx.y, tid = threadIdx.x;
-    if (first + h >= a.group) return;
-    const int head = unit / a.n_groups * a.group + first + h;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    __nv_bfloat16 *out = a.out + ((int64_t)b * a.n_q_heads + head) * D;
-    if (live_keys(a, b).y == 0) {
-        if (tid < D / 2) reinterpret_cast<uint32_t *>(out)[tid] = 0u;
-        if (a.lse && tid == 0) a.lse[(int64_t)b * a.n_q_heads + head] = -INFINITY;
-        return;
-    }
-    const int2 sp = a.split[blockIdx.x];
-    if (sp.y == 0) return;
-    // part 0 is its CTA's last unit (slot 1), the others begin their CTAs' shares (slot 0)
-    auto slot = [&](int i) { return 2 * (sp.x + i) + (i == 0); };
-    float top = -INFINITY;
-    for (int i = tid; i < sp.y; i += 256) top = fmaxf(top, a.part_ml[slot(i) * unit_heads + h].x);
-#pragma unroll
-    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    if (tid % 32 == 0) red[tid / 32] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; w++) top = fmaxf(top, red[w]);
-    float den = 0.0f;
-    for (int i = tid; i < sp.y; i += 256) {
-        const float2 ml = a.part_ml[slot(i) * unit_heads + h];
-        weight[i] = ml.x == top ? 1.0f : exp2_approx(ml.x - top);
-        den = fmaf(ml.y, weight[i], den);
-    }
-#pragma unroll
-    for (int x = 16; x; x >>= 1) den += __shfl_xor_sync(0xffffffffu, den, x);
-    if (tid % 32 == 0) dens[tid / 32] = den;
-    __syncthreads();
-    const int col = tid % kCols, row = tid / kCols;
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int i = row; i < sp.y; i += kRowsAtOnce) {
-        const float4 y = *reinterpret_cast<const float4 *>(a.part_o + ((int64_t)slot(i) * unit_heads + h) * D + col * 4);
-        const float w = weight[i];
-        sum.x = fmaf(y.x, w, sum.x); sum.y = fmaf(y.y, w, sum.y);
-        sum.z = fmaf(y.z, w, sum.z); sum.w = fmaf(y.w, w, sum.w);
-    }
-    sums[tid] = sum;
-    __syncthreads();
-    if (row) return;
-    den = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; w++) den += dens[w];
-#pragma unroll
-    for (int r = 1; r < kRowsAtOnce; r++) {
-        const float4 y = sums[r * kCols + col];
-        sum.x += y.x; sum.y += y.y; sum.z += y.z; sum.w += y.w;
-    }
-    const float inv = 1.0f / den;
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * inv, sum.y * inv),
-                         hi = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
-    reinterpret_cast<uint2 *>(out)[col] =
-        make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-    if (a.lse && tid == 0) a.lse[(int64_t)b * a.n_q_heads + head] = (top + log2f(den)) * 0.69314718f;
+    empty_streams();
 }
-
-// Workspace of a cache's attention calls, whatever their heads: two parts for every CTA of the largest
-// grid, and a split entry per unit
-constexpr int kMaxCtasPerSm = 3, kMaxUnitHeads = 16, kMaxGroups = 8;
 
 template <int D, bool I8, int NT>
 bool allow_smem() {
-    return ck(cudaFuncSetAttribute(attention_kernel<D, I8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return ck(cudaFuncSetAttribute(attention_kernel<D, I8, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   AttnShape<D, I8, NT>::kSmem),
+              "xdna_paged_cache_create") &&
+           ck(cudaFuncSetAttribute(attention_kernel<D, I8, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    AttnShape<D, I8, NT>::kSmem),
               "xdna_paged_cache_create");
 }
@@ -820,20 +996,11 @@ cudaError_t launch_attention(AttnArgs a, int sms, cudaStream_t st) {
     const int64_t units = (int64_t)a.table.n_seqs * a.pool.n_kv_heads * a.n_groups;
     int64_t keys = (int64_t)a.table.width * a.pool.page_size;
     if (a.window) keys = std::min<int64_t>(keys, a.window);
-    const int64_t tiles = units * ((keys + kTileKeys - 1) / kTileKeys);
+    const int64_t tiles = units * ((keys + kStep - 1 + kTileKeys - 1) / kTileKeys);
     const int grid = (int)std::min<int64_t>((int64_t)sms * S::kCtas, tiles);
-    attention_kernel<D, I8, NT><<<grid, 128, S::kSmem, st>>>(a);
-    if (cudaError_t e = cudaGetLastError()) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)units, std::min(a.group, S::kHeads));
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join_kernel<D>, a, (int)S::kHeads);
+    if ((tiles + 8) * (grid + 8) < 0x7fffffff) attention_kernel<D, I8, NT, true><<<grid, 128, S::kSmem, st>>>(a);
+    else attention_kernel<D, I8, NT, false><<<grid, 128, S::kSmem, st>>>(a);
+    return cudaGetLastError();
 }
 template <int D>
 cudaError_t launch_attention(const AttnArgs &a, bool i8, int sms, cudaStream_t st) {
@@ -924,7 +1091,9 @@ XdnaPagedCache *xdna_paged_cache_create(XdnaDevice *dev, const XdnaPagedCacheCon
             "xdna_paged_cache_create") ||
         !ck(cudaMalloc(&c->part_ml, (size_t)c->sms * kMaxCtasPerSm * 2 * kMaxUnitHeads * sizeof(float2)),
             "xdna_paged_cache_create") ||
-        !ck(cudaMalloc(&c->split, (size_t)g.max_seqs * g.n_kv_heads * kMaxGroups * sizeof(int2)),
+        !ck(cudaMalloc(&c->arrived, (size_t)c->sms * kMaxCtasPerSm * 2 * kJoinLevels * sizeof(int)),
+            "xdna_paged_cache_create") ||
+        !ck(cudaMemset(c->arrived, 0, (size_t)c->sms * kMaxCtasPerSm * 2 * kJoinLevels * sizeof(int)),
             "xdna_paged_cache_create") ||
         !ck(cudaMalloc(&c->status, sizeof(unsigned)), "xdna_paged_cache_create") ||
         !ck(cudaMemset(c->status, 0, sizeof(unsigned)), "xdna_paged_cache_create") ||
@@ -942,7 +1111,7 @@ void xdna_paged_cache_free(XdnaPagedCache *c) {
         cudaFree(c->status);
         cudaFree(c->part_o);
         cudaFree(c->part_ml);
-        cudaFree(c->split);
+        cudaFree(c->arrived);
     }
     delete c;
 }
@@ -1034,9 +1203,11 @@ int xdna_paged_attention(XdnaPagedCache *c, int layer, const uint16_t *q, int64_
     a.status = c->status;
     a.group = n_q_heads / g.n_kv_heads;
     a.page_shift = g.page_size & (g.page_size - 1) ? -1 : __builtin_ctz(g.page_size);
+    a.whole_steps = g.page_size % kStep == 0;
+    a.dense_steps = a.whole_steps && g.stride_slot == g.head_dim;
     a.part_o = c->part_o;
     a.part_ml = c->part_ml;
-    a.split = c->split;
+    a.arrived = c->arrived;
     auto st = static_cast<cudaStream_t>(stream);
     const bool i8 = g.kv_type != 0;
     const cudaError_t e = g.head_dim == 64    ? launch_attention<64>(a, i8, c->sms, st)

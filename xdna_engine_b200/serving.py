@@ -17,7 +17,6 @@ from . import XdnaError, _check, last_error, lib
 
 __all__ = ["PagedCache", "process_logits", "rmsnorm_residual_i8", "rope_table"]
 
-_FLOATS = (torch.bfloat16, torch.float32)
 
 
 class _PagedConfig(C.Structure):
@@ -60,28 +59,51 @@ def _lib():
     return _L
 
 
-def _want(ok, what):
-    if not ok:
-        raise ValueError(what)
-
-
-def _flat(t, dtype, shape, dev, name):
-    """The address of a contiguous tensor of exactly this type, shape and device (None: NULL)."""
+# These run in front of every launch, and a small launch is bound by them: plain attribute reads, and no
+# message is formatted unless it is raised.
+def _flat(t, dtype, n, dev, name):
+    """The address of a contiguous tensor of n elements of this type on device dev (None: NULL)."""
     if t is None:
         return None
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev.index or not t.is_contiguous():
-        raise ValueError(f"{name}: want a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}, got "
-                         f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}")
+    if t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name}: want a contiguous {dtype} tensor of {n} elements on GPU {dev}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}, strides {t.stride()}")
     return t.data_ptr()
 
 
-# the raw stream without building a torch.cuda.Stream (2 us of a small call), where torch has it
+def _heads(x, dtype, n, d, dev, name):
+    """(heads, token stride) of an [n, heads, d] tensor with contiguous heads."""
+    shape, s = x.shape, x.stride()
+    if (len(shape) != 3 or x.dtype is not dtype or shape[0] != n or shape[2] != d or s[2] != 1
+            or (s[1] != d and shape[1] != 1) or x.get_device() != dev):
+        raise ValueError(f"{name}: want {dtype} [{n}, heads, {d}] with contiguous heads on GPU {dev}, got {x.dtype} "
+                         f"{tuple(shape)} on {x.device}, strides {s}")
+    return shape[1], s[0]
+
+
+def _table(t, dev):
+    """(rows, width, row stride) of a block table."""
+    shape, s = t.shape, t.stride()
+    if len(shape) != 2 or t.dtype is not torch.int32 or (s[1] != 1 and shape[1] != 1) or t.get_device() != dev:
+        raise ValueError(f"block_table: want int32 [n_seqs, width] with contiguous rows on GPU {dev}, got {t.dtype} "
+                         f"{tuple(shape)} on {t.device}, strides {s}")
+    return shape[0], shape[1], s[0]
+
+
+def _rows(x, m, d, dev, name):
+    """Row stride of a bf16 or f32 [m, d] tensor with contiguous rows."""
+    shape, s = x.shape, x.stride()
+    if (len(shape) != 2 or shape[0] != m or shape[1] != d or (x.dtype is not torch.bfloat16 and x.dtype is not torch.float32)
+            or (s[1] != 1 and d > 1) or x.get_device() != dev):
+        raise ValueError(f"{name}: want bf16 or f32 [{m}, {d}] with contiguous rows on GPU {dev}, got {x.dtype} "
+                         f"{tuple(shape)} on {x.device}, strides {s}")
+    return s[0] if m > 1 else d
+
+
+# the raw stream and the current device without building objects (2 us of a small call), where torch has that
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def _stream(stream, dev):
-    return _raw_stream(dev.index) if stream is None else stream
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def rope_table(n_positions, rot_dim, theta=10000.0, device="cuda"):
@@ -92,18 +114,6 @@ def rope_table(n_positions, rot_dim, theta=10000.0, device="cuda"):
     return torch.cat([a.cos(), a.sin()], 1).float()
 
 
-def _is_heads(x, dtype, n, d, dev):
-    """Whether x is [n, heads, d] with contiguous heads."""
-    s, shape = x.stride(), x.shape
-    return (len(s) == 3 and x.dtype is dtype and x.get_device() == dev.index and shape[0] == n and shape[2] == d and s[2] == 1
-            and (s[1] == d or shape[1] == 1))
-
-
-def _is_table(t, dev):
-    s = t.stride()
-    return len(s) == 2 and t.dtype is torch.int32 and t.get_device() == dev.index and (s[1] == 1 or t.shape[1] == 1)
-
-
 class PagedCache:
     """A paged key-value cache over the caller's pools k and v: tensors [n_pages, n_kv_heads,
     page_size, head_dim] (or with a leading [n_layers]), bf16, or int8 with k_scale and v_scale
@@ -112,25 +122,30 @@ class PagedCache:
     one stream at a time."""
 
     def __init__(self, device, k, v, k_scale=None, v_scale=None, max_seqs=256):
-        _want(k.dim() in (4, 5) and k.shape == v.shape and k.stride() == v.stride() and k.dtype is v.dtype,
-              "k and v: want 4 or 5 dimensions and the same shape, strides and type")
-        _want(k.dtype in (torch.bfloat16, torch.int8), f"k: want bf16 or int8, got {k.dtype}")
-        _want(k.is_cuda and k.device == v.device and k.device.index == device.ordinal,
-              f"k and v are not on device {device.ordinal}")
-        _want(k.stride(-1) == 1, "k: the last dimension is not contiguous")
+        if k.dim() not in (4, 5) or k.shape != v.shape or k.stride() != v.stride() or k.dtype is not v.dtype:
+            raise ValueError("k and v: want 4 or 5 dimensions and the same shape, strides and type")
+        if k.dtype is not torch.bfloat16 and k.dtype is not torch.int8:
+            raise ValueError(f"k: want bf16 or int8, got {k.dtype}")
+        dev = device.ordinal
+        if k.get_device() != dev or v.get_device() != dev:
+            raise ValueError(f"k and v are not on device {dev}")
+        if k.stride(-1) != 1:
+            raise ValueError("k: the last dimension is not contiguous")
         i8 = k.dtype is torch.int8
-        _want(i8 == (k_scale is not None) and i8 == (v_scale is not None), "int8 pools, and only they, have scales")
+        if i8 != (k_scale is not None) or i8 != (v_scale is not None):
+            raise ValueError("int8 pools, and only they, have scales")
         five = k if k.dim() == 5 else k[None]
+        rows = k.numel() // k.shape[-1]
         c = _PagedConfig(int(i8), five.shape[0], five.shape[1], five.shape[3], five.shape[2], five.shape[4], max_seqs,
                          k.data_ptr(), v.data_ptr(), *five.stride()[:4],
-                         _flat(k_scale, torch.float32, k.shape[:-1], k.device, "k_scale"),
-                         _flat(v_scale, torch.float32, k.shape[:-1], k.device, "v_scale"))
+                         _flat(k_scale, torch.float32, rows, dev, "k_scale"),
+                         _flat(v_scale, torch.float32, rows, dev, "v_scale"))
         self.handle = None
         h = _lib().xdna_paged_cache_create(device.handle, C.byref(c))
         if not h:
             raise XdnaError(last_error())
         self.handle, self._keep = h, (k, v, k_scale, v_scale)
-        self.device, self.n_kv_heads, self.head_dim = k.device, five.shape[2], five.shape[4]
+        self.device, self.dev, self.n_kv_heads, self.head_dim = k.device, dev, five.shape[2], five.shape[4]
 
     def append(self, q, k, v, tok_seq, tok_pos, block_table, rope=None, interleaved=False, layer=0, q_out=None,
                stream=None):
@@ -139,61 +154,58 @@ class PagedCache:
         [n, heads, head_dim], all bf16 or all f32, heads contiguous, tokens at any stride; tok_seq
         (None: token t is stream t) and tok_pos int32 [n], block_table int32 [n_seqs, width], rope as
         rope_table makes it (None: no rotation)."""
-        dev, d, n = self.device, self.head_dim, tok_pos.shape[0]
-        src = k.dtype
-        _want(src in _FLOATS, f"k: want bf16 or f32, got {src}")
-        for name, x in (("q", q), ("k", k), ("v", v)):
-            if x is None and name == "q":
-                continue
-            if not _is_heads(x, src, n, d, dev):
-                raise ValueError(f"{name}: want {src} [{n}, heads, {d}] on {dev} with contiguous heads")
-        _want(k.shape[1] == self.n_kv_heads == v.shape[1], f"k and v: want {self.n_kv_heads} heads")
-        _want(_is_table(block_table, dev), "block_table: want int32 [n_seqs, width], rows contiguous")
-        hq = 0
+        dev, d, n, src = self.dev, self.head_dim, tok_pos.shape[0], k.dtype
+        if src is not torch.bfloat16 and src is not torch.float32:
+            raise ValueError(f"k: want bf16 or f32, got {src}")
+        kh, ks = _heads(k, src, n, d, dev, "k")
+        vh, vs = _heads(v, src, n, d, dev, "v")
+        if kh != self.n_kv_heads or vh != kh:
+            raise ValueError(f"k and v: want {self.n_kv_heads} heads, got {kh} and {vh}")
+        hq = qs = rows = rot = 0
         if q is not None:
-            hq = q.shape[1]
+            hq, qs = _heads(q, src, n, d, dev, "q")
             if q_out is None:
-                q_out = torch.empty(n, hq, d, dtype=torch.bfloat16, device=dev)
-        rows = rot = 0
+                q_out = torch.empty(n, hq, d, dtype=torch.bfloat16, device=self.device)
         if rope is not None:
             rows, rot = rope.shape
+        n_seqs, width, ts = _table(block_table, dev)
         if n == 0:
             return q_out
-        _check(_lib().xdna_paged_append(
-            self.handle, layer, n, hq, src is torch.float32,
-            None if q is None else q.data_ptr(), 0 if q is None else q.stride(0), k.data_ptr(), k.stride(0),
-            v.data_ptr(), v.stride(0), _flat(tok_seq, torch.int32, (n,), dev, "tok_seq"),
-            _flat(tok_pos, torch.int32, (n,), dev, "tok_pos"), block_table.data_ptr(), block_table.shape[0],
-            block_table.shape[1], block_table.stride(0),
-            None if rope is None else _flat(rope, torch.float32, rope.shape, dev, "rope"), rows, rot, interleaved,
-            None if q is None else _flat(q_out, torch.bfloat16, (n, hq, d), dev, "q_out"), _stream(stream, dev)))
+        if (_L or _lib()).xdna_paged_append(
+                self.handle, layer, n, hq, src is torch.float32, None if q is None else q.data_ptr(), qs, k.data_ptr(),
+                ks, v.data_ptr(), vs, _flat(tok_seq, torch.int32, n, dev, "tok_seq"),
+                _flat(tok_pos, torch.int32, n, dev, "tok_pos"), block_table.data_ptr(), n_seqs, width, ts,
+                _flat(rope, torch.float32, rows * rot, dev, "rope"), rows, rot, interleaved,
+                None if q is None else _flat(q_out, torch.bfloat16, n * hq * d, dev, "q_out"),
+                _raw_stream(dev) if stream is None else stream):
+            raise XdnaError(last_error())
         return q_out
 
     def attend(self, q, block_table, seq_lens, scale=None, window=0, layer=0, out=None, lse=None, stream=None):
         """Attention of one new token per stream, q bf16 [n_seqs, n_q_heads, head_dim], over the last
         `window` (0: all) of its seq_lens[b] positions; scale None: head_dim ** -0.5.  Returns out
         (bf16, as q); lse (f32 [n_seqs, n_q_heads]) is filled when given."""
-        dev, d, n = self.device, self.head_dim, seq_lens.shape[0]
-        if not _is_heads(q, torch.bfloat16, n, d, dev):
-            raise ValueError(f"q: want bf16 [{n}, heads, {d}] on {dev} with contiguous heads")
-        _want(_is_table(block_table, dev) and block_table.shape[0] == n,
-              "block_table: want int32 [n_seqs, width], rows contiguous")
-        hq = q.shape[1]
+        dev, d, n = self.dev, self.head_dim, seq_lens.shape[0]
+        hq, qs = _heads(q, torch.bfloat16, n, d, dev, "q")
+        n_seqs, width, ts = _table(block_table, dev)
+        if n_seqs != n:
+            raise ValueError(f"block_table: want {n} rows, got {n_seqs}")
         if out is None:
-            out = torch.empty(n, hq, d, dtype=torch.bfloat16, device=dev)
+            out = torch.empty(n, hq, d, dtype=torch.bfloat16, device=self.device)
         if n == 0:
             return out
-        _check(_lib().xdna_paged_attention(
-            self.handle, layer, q.data_ptr(), q.stride(0) if n > 1 else hq * d, hq, block_table.data_ptr(), n,
-            block_table.shape[1], block_table.stride(0), _flat(seq_lens, torch.int32, (n,), dev, "seq_lens"),
-            d ** -0.5 if scale is None else scale, window, _flat(out, torch.bfloat16, (n, hq, d), dev, "out"),
-            _flat(lse, torch.float32, (n, hq), dev, "lse"), _stream(stream, dev)))
+        if (_L or _lib()).xdna_paged_attention(
+                self.handle, layer, q.data_ptr(), qs if n > 1 else hq * d, hq, block_table.data_ptr(), n, width, ts,
+                _flat(seq_lens, torch.int32, n, dev, "seq_lens"), d ** -0.5 if scale is None else scale, window,
+                _flat(out, torch.bfloat16, n * hq * d, dev, "out"), _flat(lse, torch.float32, n * hq, dev, "lse"),
+                _raw_stream(dev) if stream is None else stream):
+            raise XdnaError(last_error())
         return out
 
     def check(self, stream=None):
         """Wait for the stream and raise XdnaError for page ids, positions or streams out of range
         that calls since the last check met."""
-        _check(_lib().xdna_paged_cache_check(self.handle, _stream(stream, self.device)))
+        _check(_lib().xdna_paged_cache_check(self.handle, _raw_stream(self.dev) if stream is None else stream))
 
     def close(self):
         if getattr(self, "handle", None):
@@ -207,14 +219,6 @@ class PagedCache:
             pass
 
 
-def _rows(x, m, d, dev, name):
-    """Row stride of an [m, d] tensor with contiguous rows."""
-    s = x.stride()
-    if x.shape != (m, d) or x.dtype not in _FLOATS or x.get_device() != dev.index or (s[1] != 1 and d > 1):
-        raise ValueError(f"{name}: want bf16 or f32 [{m}, {d}] on {dev}, rows contiguous")
-    return s[0] if m > 1 else d
-
-
 def rmsnorm_residual_i8(x, gamma, residual=None, eps=1e-6, unit_offset=False, q8=None, scale=None, residual_out=None,
                         y=None, quantize=True, stream=None):
     """r = x + residual; y = r / sqrt(mean(r^2) + eps) * gamma (gamma + 1 with unit_offset), as int8
@@ -222,38 +226,42 @@ def rmsnorm_residual_i8(x, gamma, residual=None, eps=1e-6, unit_offset=False, q8
     residual_out): residual_out holds r in residual's type (None without a residual); a given buffer is
     used, residual itself among them.  `y` (bf16 [m, d]) also takes the unquantised norm;
     quantize=False leaves q8 and scale out (None)."""
-    _want(x.dim() == 2 and x.is_cuda, "x: want [m, d] on a GPU")
-    dev, (m, d) = x.device, x.shape
+    dev = x.get_device()
+    if dev < 0 or x.dim() != 2:
+        raise ValueError(f"x: want [m, d] on a GPU, got {tuple(x.shape)} on {x.device}")
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return rmsnorm_residual_i8(x, gamma, residual, eps, unit_offset, q8, scale, residual_out, y, quantize, stream)
+    m, d = x.shape
     xs = _rows(x, m, d, dev, "x")
     rs = 0
+    res_f32 = False
     if residual is not None:
         rs = _rows(residual, m, d, dev, "residual")
+        res_f32 = residual.dtype is torch.float32
         if residual_out is None:
-            residual_out = torch.empty_strided((m, d), (rs, 1), dtype=residual.dtype, device=dev)
-        _want(residual_out.dtype is residual.dtype and _rows(residual_out, m, d, dev, "residual_out") == rs,
-              "residual_out: want the type and row stride of residual")
-    else:
-        _want(residual_out is None, "residual_out without a residual")
+            residual_out = torch.empty_strided((m, d), (rs, 1), dtype=residual.dtype, device=x.device)
+        elif residual_out is not residual and (
+                residual_out.dtype is not residual.dtype or _rows(residual_out, m, d, dev, "residual_out") != rs):
+            raise ValueError("residual_out: want the type and row stride of residual")
+    elif residual_out is not None:
+        raise ValueError("residual_out without a residual")
     if quantize:
         if q8 is None:
-            q8 = torch.empty(m, d, dtype=torch.int8, device=dev)
+            q8 = torch.empty(m, d, dtype=torch.int8, device=x.device)
         if scale is None:
-            scale = torch.empty(m, dtype=torch.float32, device=dev)
-    else:
-        _want(q8 is None and scale is None, "q8 or scale with quantize=False")
+            scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    elif q8 is not None or scale is not None:
+        raise ValueError("q8 or scale with quantize=False")
     if m == 0:
         return q8, scale, residual_out
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            rmsnorm_residual_i8(x, gamma, residual, eps, unit_offset, q8, scale, residual_out, y, quantize, stream)
-    else:
-        _check(_lib().xdna_rmsnorm_residual_i8(
-            x.data_ptr(), x.dtype is torch.float32, xs, None if residual is None else residual.data_ptr(),
-            residual is not None and residual.dtype is torch.float32, rs,
-            _flat(gamma, torch.float32, (d,), dev, "gamma"), unit_offset, eps, m, d,
-            None if residual_out is None else residual_out.data_ptr(),
-            _flat(y, torch.bfloat16, (m, d), dev, "y"), _flat(q8, torch.int8, (m, d), dev, "q8"),
-            _flat(scale, torch.float32, (m,), dev, "scale"), _stream(stream, dev)))
+    if (_L or _lib()).xdna_rmsnorm_residual_i8(
+            x.data_ptr(), x.dtype is torch.float32, xs, None if residual is None else residual.data_ptr(), res_f32, rs,
+            _flat(gamma, torch.float32, d, dev, "gamma"), unit_offset, eps, m, d,
+            None if residual_out is None else residual_out.data_ptr(), _flat(y, torch.bfloat16, m * d, dev, "y"),
+            _flat(q8, torch.int8, m * d, dev, "q8"), _flat(scale, torch.float32, m, dev, "scale"),
+            _raw_stream(dev) if stream is None else stream):
+        raise XdnaError(last_error())
     return q8, scale, residual_out
 
 
@@ -265,36 +273,38 @@ def process_logits(logits, history=None, history_start=None, n_prompt=None, repe
     mask leaves none).  history int32 [total] with history_start int32 [b + 1]; n_prompt int32 [b];
     repetition, frequency, presence f32 [b]; bias_ids int32, bias f32 [entries] with bias_start int32
     [b + 1]; mask int32 [b, (v + 31) / 32], bit set: allowed.  out may be logits (f32)."""
-    _want(logits.dim() == 2 and logits.is_cuda, "logits: want [b, v] on a GPU")
-    dev, (b, v) = logits.device, logits.shape
+    dev = logits.get_device()
+    if dev < 0 or logits.dim() != 2:
+        raise ValueError(f"logits: want [b, v] on a GPU, got {tuple(logits.shape)} on {logits.device}")
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return process_logits(logits, history, history_start, n_prompt, repetition, frequency, presence, bias_ids,
+                                  bias, bias_start, mask, out, ids, stream)
+    b, v = logits.shape
+    i32, f32 = torch.int32, torch.float32
     ls = _rows(logits, b, v, dev, "logits")
     if out is None:
-        out = torch.empty(b, v, dtype=torch.float32, device=dev)
+        out = torch.empty(b, v, dtype=f32, device=logits.device)
     os_ = _rows(out, b, v, dev, "out")
-    _want(out.dtype is torch.float32, "out: want f32")
+    if out.dtype is not f32:
+        raise ValueError(f"out: want f32, got {out.dtype}")
     if ids is None:
-        ids = torch.empty(b, dtype=torch.int64, device=dev)
+        ids = torch.empty(b, dtype=torch.int64, device=logits.device)
     if b == 0:
         return out, ids
-    i32, f32 = torch.int32, torch.float32
-    _want(history is None or history.dim() == 1, "history: want one dimension")
-    _want(bias is None or bias.dim() == 1, "bias: want one dimension")
-    work = _lib().xdna_logits_workspace(b, v)
-    work = torch.empty(work, dtype=torch.uint8, device=dev) if work else None
-    n = 0 if history is None else history.shape[0]
-    e = 0 if bias is None else bias.shape[0]
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            process_logits(logits, history, history_start, n_prompt, repetition, frequency, presence, bias_ids, bias,
-                           bias_start, mask, out, ids, stream)
-    else:
-        _check(_lib().xdna_logits_process(
-            logits.data_ptr(), logits.dtype is f32, ls, b, v, _flat(history, i32, (n,), dev, "history"), n,
-            _flat(history_start, i32, (b + 1,), dev, "history_start"), _flat(n_prompt, i32, (b,), dev, "n_prompt"),
-            _flat(repetition, f32, (b,), dev, "repetition"), _flat(frequency, f32, (b,), dev, "frequency"),
-            _flat(presence, f32, (b,), dev, "presence"), _flat(bias_ids, i32, (e,), dev, "bias_ids"),
-            _flat(bias, f32, (e,), dev, "bias"), e, _flat(bias_start, i32, (b + 1,), dev, "bias_start"),
-            _flat(mask, i32, (b, (v + 31) // 32), dev, "mask"), (v + 31) // 32, out.data_ptr(), os_,
-            _flat(ids, torch.int64, (b,), dev, "ids"), None if work is None else work.data_ptr(),
-            _stream(stream, dev)))
+    L = _L or _lib()
+    # rows of several clusters of CTAs need room for their chunks' choices
+    work = torch.empty(L.xdna_logits_workspace(b, v), dtype=torch.uint8, device=logits.device) if v > 60000 else None
+    n = 0 if history is None else history.numel()
+    e = 0 if bias is None else bias.numel()
+    words = (v + 31) // 32
+    if L.xdna_logits_process(
+            logits.data_ptr(), logits.dtype is f32, ls, b, v, _flat(history, i32, n, dev, "history"), n,
+            _flat(history_start, i32, b + 1, dev, "history_start"), _flat(n_prompt, i32, b, dev, "n_prompt"),
+            _flat(repetition, f32, b, dev, "repetition"), _flat(frequency, f32, b, dev, "frequency"),
+            _flat(presence, f32, b, dev, "presence"), _flat(bias_ids, i32, e, dev, "bias_ids"),
+            _flat(bias, f32, e, dev, "bias"), e, _flat(bias_start, i32, b + 1, dev, "bias_start"),
+            _flat(mask, i32, b * words, dev, "mask"), words, out.data_ptr(), os_, _flat(ids, torch.int64, b, dev, "ids"),
+            None if work is None else work.data_ptr(), _raw_stream(dev) if stream is None else stream):
+        raise XdnaError(last_error())
     return out, ids
