@@ -225,11 +225,14 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 //
 // Work split.  A unit is (stream, K/V head, group of up to 8 NT query heads); its keys are cut into
 // tiles of 16 keys per warp.  All units' tiles, laid end to end, are dealt to the CTAs in equal
-// contiguous shares, whatever the streams' lengths; a CTA walks its share unit by unit.  A unit
+// contiguous shares, whatever the streams' lengths; a CTA walks its share unit by unit.  A unit's end
+// counts as kEndCost tiles, since its work there costs so much (32 ragged streams of 12 heads x 64, up
+// to 2k: 32.2 us at 0, 29.5 at 1, 27.4 at 2, 27.2 at 3).  A unit
 // that lies in one CTA is written at once; of one that shares' borders cut, each CTA leaves its
 // (max, sum, unnormalised o) in the workspace, and the last of every 16 neighbours to do so adds
-// theirs, in CTA order whoever is last, until one is left: no CTA waits, no second launch.  A fence, an atomic and a part's way through L2 take about 3 us, as long as some 4 tiles: a small call
-// gets fewer CTAs, so that a unit has no more than 16 parts, or exactly as many a unit.
+// theirs, in CTA order whoever is last, until one is left: no CTA waits, no second launch.  A fence, an
+// atomic and a part's way through L2 take about 3 us, as long as some 4 tiles: a small call gets
+// fewer CTAs, so that a unit has no more than 16 parts, or equally many CTAs a unit.
 //
 // Inside a CTA each warp runs alone: its own ring of cp.async stages (16 keys' K and V rows), which
 // runs on over the share's units without a break, its own running maximum and sum, no barrier
@@ -272,6 +275,7 @@ struct AttnShape {
     static constexpr int kStages = kRows >= 8192 ? 3 : kRows >= 4096 ? 4 : 6;
     static constexpr int kStage = kRows + (I8 ? 128 : 0) + 16;           // + scales, + live mask
     static constexpr int kHeads = 8 * NT;
+    static constexpr int kEndCost = 2, kApartTiles = 4;
     static constexpr int kRing = kWarps * kStages * kStage;
     static constexpr int kJoinCols = 32, kJoinRow = kJoinCols + 4;
     static constexpr int kJoin = kWarps * kHeads * kJoinRow * 4;
@@ -391,59 +395,83 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
         }
     };
 
-    // ---- this CTA's share: tiles [share0, share1) of all units laid end to end.  Every warp works it out
-    // for itself, 128 streams at a time, 4 to a lane.
+    // ---- this CTA's share: [share0, share1) of all units' tiles and ends laid end to end.  Every warp works
+    // it out for itself, 128 streams at a time, 4 to a lane.
     const int units_per_stream = a.pool.n_kv_heads * a.n_groups, B = a.table.n_seqs;
-    int tiles4[4], mine = 0, upto = 0;                    // a lane's streams, their sum, the sum up to them
+    int tiles4[4], mine = 0, upto = 0;                    // of a lane's streams, their sum, the sum up to them
+    int some = 0, some_upto = 0;                          // the same for how many have any
     auto count128 = [&](int b0) {
-        mine = 0;
+        mine = some = 0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int b = b0 + lane * 4 + k;
-            mine += tiles4[k] = b < B ? live_keys(a, a.lens[b]).tiles : 0;
+            tiles4[k] = b < B ? live_keys(a, a.lens[b]).tiles : 0;
+            mine += tiles4[k];
+            some += tiles4[k] != 0;
         }
         upto = mine;
+        some_upto = some;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
-            const int y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
+            const int y = __shfl_up_sync(0xffffffffu, upto, o), z = __shfl_up_sync(0xffffffffu, some_upto, o);
+            if (lane >= o) {
+                upto += y;
+                some_upto += z;
+            }
         }
-        return __shfl_sync(0xffffffffu, upto, 31);
     };
     using Int = std::conditional_t<kSmall, int, int64_t>;  // total * ctas fits
-    Int total = 0;
-    for (int b0 = 0; b0 < B; b0 += 128) total += count128(b0);
+    Int total = 0, live_units = 0;
+    int longest = 0;
+    for (int b0 = 0; b0 < B; b0 += 128) {
+        count128(b0);
+        total += __shfl_sync(0xffffffffu, upto, 31);
+        live_units += __shfl_sync(0xffffffffu, some_upto, 31);
+        longest = max(longest, __reduce_max_sync(0xffffffffu, max(max(tiles4[0], tiles4[1]), max(tiles4[2], tiles4[3]))));
+    }
     total *= units_per_stream;
+    live_units *= units_per_stream;
     if (total == 0) {
         empty_streams();
         return;
     }
-    // no share is empty, so that a unit's parts lie in consecutive CTAs
-    const Int units = (Int)B * units_per_stream;
+    // Short units, one CTA to each: what is left then to join within it takes less than parts would.  Else no
+    // share is empty, so that a unit's parts lie in consecutive CTAs (one may hold an end alone): up to 64
+    // tiles a unit, no more CTAs than make 16 parts of the longest; units of one length and few tiles,
+    // as many CTAs to each, whose parts then all have an end
+    const bool apart = live_units <= (Int)gridDim.x && longest <= S::kApartTiles;
     Int want = min((Int)gridDim.x, total);
-    if (total <= units * (4 * kJoinWays)) want = min(want, units * kJoinWays);
-    if (units < want && total < 8 * want) want = want / units * units;
-    const int ctas = (int)want;
+    if (longest <= 4 * kJoinWays) want = min(want, total * kJoinWays / longest);
+    const bool even = live_units < want && total < 8 * want && (Int)longest * live_units == total;
+    if (even) want = want / live_units * live_units;
+    const int ctas = (int)(apart ? live_units : want), end_cost = even ? 0 : S::kEndCost;
     if ((int)blockIdx.x >= ctas) {
         empty_streams();
         return;
     }
-    const Int share0 = total * (Int)blockIdx.x / ctas, share1 = total * (Int)(blockIdx.x + 1) / ctas;
+    total += live_units * end_cost;
+    const Int share0 = apart ? (Int)blockIdx.x : total * (Int)blockIdx.x / ctas;
+    const Int share1 = apart ? share0 + 1 : total * (Int)(blockIdx.x + 1) / ctas;
     int at_b = 0, at_unit = 0, at_tile = 0;
-    Int before = 0;                                       // tiles of one head of the streams before b0
+    Int before = 0;                                       // what the streams before b0 come to
     for (int b0 = 0; b0 < B; b0 += 128) {
-        const int sum = B > 128 ? count128(b0) : 0;
-        if (B <= 128 || (before + sum) * units_per_stream > share0) {
-            Int from = (before + upto - mine) * units_per_stream;
-            const bool here = mine && from <= share0 && share0 < from + (Int)mine * units_per_stream;
-            int k = 0, n = max(1, tiles4[0]);
+        if (B > 128) count128(b0);
+        // what a lane's streams come to, of one unit each: in tiles and ends, or in units
+        const Int own = apart ? (Int)some : mine + (Int)some * end_cost;
+        const Int upto_own = apart ? (Int)some_upto : upto + (Int)some_upto * end_cost;
+        const Int sum = __shfl_sync(0xffffffffu, upto_own, 31);
+        if (before + sum * units_per_stream > share0) {
+            Int from = before + (upto_own - own) * units_per_stream;
+            const bool here = own && from <= share0 && share0 < from + own * units_per_stream;
+            auto unit_of = [&](int q) { return tiles4[q] == 0 ? 0 : apart ? 1 : tiles4[q] + end_cost; };
+            int k = 0, n = max(1, unit_of(0));
 #pragma unroll
             for (int q = 0; q < 3; q++) {
-                const Int next = from + (Int)tiles4[q] * units_per_stream;
+                const Int next = from + (Int)unit_of(q) * units_per_stream;
                 if (k == q && share0 >= next) {
                     from = next;
                     k = q + 1;
-                    n = max(1, tiles4[q + 1]);
+                    n = max(1, unit_of(q + 1));
                 }
             }
             const Int off = here ? share0 - from : 0;
@@ -454,7 +482,7 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
             at_tile = __shfl_sync(0xffffffffu, tile, owner);
             break;
         }
-        before += sum;
+        before += sum * units_per_stream;
     }
 
     // ---- a place in the share: a unit of a stream, and a tile of its keys
@@ -473,7 +501,23 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
         }
     };
     Place at{at_b, at_unit, at_tile, live_keys(a, a.lens[at_b])}, ahead = at;
-    int left = (int)(share1 - share0), unfetched = left;
+    int left = apart ? at.live.tiles : (int)(share1 - share0), unfetched = left;
+    Int unit_at = share0 - at.t;                          // where the unit begins
+    auto pass_end = [&](Place &p, int &rest) {            // from a unit's last tile to the next unit, if the share goes on
+        rest -= end_cost;
+        if (rest > 0) next_unit(p);
+    };
+    if (at.t >= at.live.tiles) {                          // the share begins in a unit's end
+        unit_at += at.live.tiles + end_cost;
+        left -= (int)(unit_at - share0) - end_cost;
+        pass_end(at, left);
+        if (left <= 0) {
+            empty_streams();
+            return;
+        }
+        ahead = at;
+        unfetched = left;
+    }
 
     // ---- the ring.  issue() copies the step of the place `ahead`, whose page (that of its key r in lanes r
     // and r + 16, where steps do not lie whole in pages) look_up() fetched a step before, and moves on.
@@ -532,9 +576,9 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
             }
         }
         if (lane == 0) *reinterpret_cast<unsigned *>(ring + stage * S::kStage + S::kStage - 16) = mask;
-        if (--unfetched == 0) return;
+        unfetched--;
         if (++ahead.t == ahead.live.tiles) {
-            next_unit(ahead);
+            pass_end(ahead, unfetched);
             ahead_hk = ahead.unit / a.n_groups;
         }
     };
@@ -779,11 +823,13 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
 
         // ---- the unit's end: the warps' parts into one, the next unit's q on its way meanwhile
         const Place done = at;
+        const Int begin = unit_at;
         left -= run;
-        if (left) {
-            next_unit(at);
-            load_q(at);
+        if (left > 0) {                                   // else the unit may go on in the next share
+            unit_at += at.live.tiles + end_cost;
+            pass_end(at, left);
         }
+        if (left > 0) load_q(at);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -796,9 +842,9 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
                     join_l[warp][nt * 8 + 2 * j + i] = l[nt][i];
                 }
             }
-        if (!left) xdna::cp_async_wait_all();
+        if (left <= 0) xdna::cp_async_wait_all();
         __syncthreads();
-        if (left) store_q();
+        if (left > 0) store_q();
         const int hk = done.unit / a.n_groups, h0 = hk * a.group + (done.unit % a.n_groups) * S::kHeads;
         const int heads = min(S::kHeads, a.group - (done.unit % a.n_groups) * S::kHeads);
         const bool whole = done.t == 0 && run == done.live.tiles;
@@ -861,7 +907,7 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
                 }
             }
         };
-        if (left) {
+        if (left > 0) {
             join_warps(std::integral_constant<int, S::kJoinCols>{});
         } else {                                          // the ring is free: all at once
             join_o = reinterpret_cast<float *>(smem);
@@ -877,7 +923,6 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
             // ---- parts: a unit's tiles [begin, begin + tiles) lie in the shares of CTAs first .. first + parts - 1
             __threadfence();
             __syncthreads();
-            const Int begin = share1 - left - run - done.t;
             const int first = (int)(((begin + 1) * ctas - 1) / total);
             const int parts = (int)(((begin + done.live.tiles) * ctas - 1) / total) - first + 1;
             for (int level = 0, n = parts, i = blockIdx.x - first, stride = 1; level < kJoinLevels; level++) {
@@ -966,7 +1011,7 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
                 stride *= kJoinWays;
             }
         }
-        if (!left) break;
+        if (left <= 0) break;
         __syncthreads();
         take_q();
     }
@@ -996,7 +1041,7 @@ cudaError_t launch_attention(AttnArgs a, int sms, cudaStream_t st) {
     const int64_t units = (int64_t)a.table.n_seqs * a.pool.n_kv_heads * a.n_groups;
     int64_t keys = (int64_t)a.table.width * a.pool.page_size;
     if (a.window) keys = std::min<int64_t>(keys, a.window);
-    const int64_t tiles = units * ((keys + kStep - 1 + kTileKeys - 1) / kTileKeys);
+    const int64_t tiles = units * ((keys + kStep - 1 + kTileKeys - 1) / kTileKeys + S::kEndCost);
     const int grid = (int)std::min<int64_t>((int64_t)sms * S::kCtas, tiles);
     if ((tiles + 8) * (grid + 8) < 0x7fffffff) attention_kernel<D, I8, NT, true><<<grid, 128, S::kSmem, st>>>(a);
     else attention_kernel<D, I8, NT, false><<<grid, 128, S::kSmem, st>>>(a);
