@@ -38,7 +38,7 @@ struct NormArgs {
     const void *x, *res;
     int64_t x_stride, res_stride;
     const float *gamma;
-    int unit_offset, D;
+    int unit_offset, M, D;
     float eps;
     void *res_out;
     __nv_bfloat16 *y;
@@ -46,31 +46,39 @@ struct NormArgs {
     float *scale;
 };
 
-// N elements of a row as f32 (8: one or two 16-byte loads)
-template <int N>
-__device__ __forceinline__ void load_n(const float *p, float (&v)[N]) {
-    if constexpr (N == 8) {
-        const float4 a = __ldcs(reinterpret_cast<const float4 *>(p)), b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        v[0] = __ldcs(p);
+// N elements of a row as they lie in memory (8: one or two 16-byte loads), and as f32
+template <typename T, int N>
+struct Piece;
+template <>
+struct Piece<float, 8> {
+    float4 a, b;
+    __device__ void load(const float *p) {
+        a = __ldcs(reinterpret_cast<const float4 *>(p));
+        b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
     }
-}
-template <int N>
-__device__ __forceinline__ void load_n(const __nv_bfloat16 *p, float (&v)[N]) {
-    if constexpr (N == 8) {
-        const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(p));
-        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[2 * i] = xdna::bf16lo(u[i]);
-            v[2 * i + 1] = xdna::bf16hi(u[i]);
-        }
-    } else {
-        v[0] = __bfloat162float(*p);
+    __device__ float operator[](int k) const { return k == 0 ? a.x : k == 1 ? a.y : k == 2 ? a.z : k == 3 ? a.w : k == 4 ? b.x : k == 5 ? b.y : k == 6 ? b.z : b.w; }
+};
+template <>
+struct Piece<__nv_bfloat16, 8> {
+    uint4 a;
+    __device__ void load(const __nv_bfloat16 *p) { a = __ldcs(reinterpret_cast<const uint4 *>(p)); }
+    __device__ float operator[](int k) const {
+        const uint32_t u = k < 2 ? a.x : k < 4 ? a.y : k < 6 ? a.z : a.w;
+        return k % 2 ? xdna::bf16hi(u) : xdna::bf16lo(u);
     }
-}
+};
+template <>
+struct Piece<float, 1> {
+    float a;
+    __device__ void load(const float *p) { a = __ldcs(p); }
+    __device__ float operator[](int) const { return a; }
+};
+template <>
+struct Piece<__nv_bfloat16, 1> {
+    __nv_bfloat16 a;
+    __device__ void load(const __nv_bfloat16 *p) { a = *p; }
+    __device__ float operator[](int) const { return __bfloat162float(a); }
+};
 template <int N>
 __device__ __forceinline__ void store_n(float *p, const float (&v)[N]) {
     if constexpr (N == 8) {
@@ -85,122 +93,152 @@ __device__ __forceinline__ void store_n(__nv_bfloat16 *p, const float (&v)[N]) {
     if constexpr (N == 8) {
         uint32_t u[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) u[i] = xdna::bf16bits(v[2 * i]) | (xdna::bf16bits(v[2 * i + 1]) << 16);
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            u[i] = *reinterpret_cast<const uint32_t *>(&two);
+        }
         *reinterpret_cast<uint4 *>(p) = make_uint4(u[0], u[1], u[2], u[3]);
     } else {
         *p = __float2bfloat16_rn(v[0]);
     }
 }
 
-// One CTA per row, one pass: a thread keeps P pieces of N elements in registers, so that x and the
-// residual are read once (7 bytes an element with bf16 in and out: HBM bounds it); the sum of squares and
-// max|r g| need one joint reduction, since the row's factor 1 / rms scales both y and its maximum and
-// drops out of the whole numbers.  N = 8 where every row is 16-byte aligned, else N = 1.
-template <typename X, typename R, int N, int P>
-__global__ void __launch_bounds__(1024) rmsnorm_kernel(const NormArgs a) {
-    __shared__ float red[2][32];
-    const int64_t row = blockIdx.x;
-    const X *x = static_cast<const X *>(a.x) + row * a.x_stride;
-    const R *res = a.res ? static_cast<const R *>(a.res) + row * a.res_stride : nullptr;
-    const int threads = blockDim.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    float r[P][N];
-#pragma unroll
-    for (int p = 0; p < P; p++) {
-        const int i = (p * threads + threadIdx.x) * N;
-        if (i < a.D) {
-            load_n(x + i, r[p]);
-            if (res) {
-                float y[N];
-                load_n(res + i, y);
-#pragma unroll
-                for (int k = 0; k < N; k++) r[p][k] = __fadd_rn(r[p][k], y[k]);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < N; k++) r[p][k] = 0.0f;
-        }
-    }
-    float sum = 0.0f, top = 0.0f;
-#pragma unroll
-    for (int p = 0; p < P; p++) {
-        const int i = (p * threads + threadIdx.x) * N;
-        if (i >= a.D) break;
-        if (a.res_out) store_n(static_cast<R *>(a.res_out) + row * a.res_stride + i, r[p]);
-        float w[N];
+// A CTA takes every gridDim.x-th row, one pass over it: a thread keeps P pieces of N elements in
+// registers, so that x and the residual are read once (7 bytes an element with bf16 in and out: HBM
+// bounds it).  The sum of squares and max|r g| need one joint reduction, since the row's factor 1 / rms
+// scales both y and its maximum and drops out of the whole numbers.  kAhead: gamma stays in registers and
+// the next row's loads pass under the reduction and the outputs; without it (wide rows, whose
+// threads have no registers left) other CTAs of the SM do that.  N = 8 where every row is 16-byte
+// aligned, else N = 1.
+template <typename X, typename R, int N, int P, int kThreads, bool kAhead>
+__global__ void __launch_bounds__(kThreads) rmsnorm_kernel(const NormArgs a) {
+    __shared__ float2 red[2][kThreads / 32];              // alternating, so that a row needs one barrier
+    const int threads = blockDim.x, warps = threads / 32, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    auto place = [&](int p) { return (p * threads + (int)threadIdx.x) * N; };
+    Piece<X, N> x[kAhead ? P : 1];
+    Piece<R, N> res[kAhead ? P : 1];
+    auto load = [&](int64_t row, int p, int to) {
+        if (place(p) >= a.D) return;
+        x[to].load(static_cast<const X *>(a.x) + row * a.x_stride + place(p));
+        if (a.res) res[to].load(static_cast<const R *>(a.res) + row * a.res_stride + place(p));
+    };
+    float g[kAhead ? P : 1][N];
+    auto load_gamma = [&](int p, float (&w)[N]) {
         if constexpr (N == 8) {
-            const float4 lo = __ldg(reinterpret_cast<const float4 *>(a.gamma + i)),
-                         hi = __ldg(reinterpret_cast<const float4 *>(a.gamma + i) + 1);
+            const float4 lo = __ldg(reinterpret_cast<const float4 *>(a.gamma + place(p))),
+                         hi = __ldg(reinterpret_cast<const float4 *>(a.gamma + place(p)) + 1);
             w[0] = lo.x; w[1] = lo.y; w[2] = lo.z; w[3] = lo.w;
             w[4] = hi.x; w[5] = hi.y; w[6] = hi.z; w[7] = hi.w;
         } else {
-            w[0] = __ldg(a.gamma + i);
+            w[0] = __ldg(a.gamma + place(p));
+        }
+        if (a.unit_offset)
+#pragma unroll
+            for (int k = 0; k < N; k++) w[k] = __fadd_rn(w[k], 1.0f);
+    };
+    if constexpr (kAhead) {
+#pragma unroll
+        for (int p = 0; p < P; p++) load(blockIdx.x, p, p);
+#pragma unroll
+        for (int p = 0; p < P; p++)
+            if (place(p) < a.D) load_gamma(p, g[p]);
+    }
+    int phase = 0;
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x, phase ^= 1) {
+        float r[P][N], sum = 0.0f, top = 0.0f;
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            if (place(p) >= a.D) break;
+            if (!kAhead) load(row, p, 0);
+            const int at = kAhead ? p : 0;
+#pragma unroll
+            for (int k = 0; k < N; k++) r[p][k] = a.res ? __fadd_rn(x[at][k], res[at][k]) : x[at][k];
+        }
+        if (kAhead && row + gridDim.x < a.M) {
+#pragma unroll
+            for (int p = 0; p < P; p++) load(row + gridDim.x, p, kAhead ? p : 0);
         }
 #pragma unroll
-        for (int k = 0; k < N; k++) {
-            const float g = a.unit_offset ? __fadd_rn(w[k], 1.0f) : w[k];
-            sum = fmaf(r[p][k], r[p][k], sum);
-            r[p][k] = __fmul_rn(r[p][k], g);
-            top = fmaxf(top, fabsf(r[p][k]));
+        for (int p = 0; p < P; p++) {
+            if (place(p) >= a.D) break;
+            if (a.res_out) store_n(static_cast<R *>(a.res_out) + row * a.res_stride + place(p), r[p]);
+            float w[N];
+            if constexpr (!kAhead) load_gamma(p, w);
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                sum = fmaf(r[p][k], r[p][k], sum);
+                r[p][k] = __fmul_rn(r[p][k], kAhead ? g[p][k] : w[k]);
+                top = fmaxf(top, fabsf(r[p][k]));
+            }
         }
-    }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    }
-    if (lane == 0) {
-        red[0][warp] = sum;
-        red[1][warp] = top;
-    }
-    __syncthreads();
-    sum = lane < threads / 32 ? red[0][lane] : 0.0f;
-    top = lane < threads / 32 ? red[1][lane] : 0.0f;
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));   // not negative: ordered as bits
+        if (lane == 0) red[phase][warp] = make_float2(sum, top);
+        __syncthreads();
+        if constexpr (kThreads <= 256) {
+            sum = red[phase][0].x;
+            for (int w = 1; w < warps; w++) {
+                sum += red[phase][w].x;
+                top = fmaxf(top, red[phase][w].y);
+            }
+            top = fmaxf(top, red[phase][0].y);
+        } else {
+            const float2 part = lane < warps ? red[phase][lane] : make_float2(0.0f, 0.0f);
+            sum = part.x;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    }
-    const float inv = rsqrtf(__fdiv_rn(sum, (float)a.D) + a.eps);
-    // below 127 / FLT_MAX the factor would be infinite: such a row counts as zero
-    const bool zero = !(top > 3.8e-37f);
-    const float to8 = zero ? 0.0f : __fmul_rn(__frcp_rn(top), 127.0f);
-#pragma unroll
-    for (int p = 0; p < P; p++) {
-        const int i = (p * threads + threadIdx.x) * N;
-        if (i >= a.D) break;
-        if (a.q8) {
-            uint32_t w[N == 8 ? 2 : 1] = {};
-#pragma unroll
-            for (int k = 0; k < N; k++)
-                w[k / 4] |= ((uint32_t)max(-127, min(127, __float2int_rn(__fmul_rn(r[p][k], to8)))) & 0xffu) << (8 * (k % 4));
-            if constexpr (N == 8) *reinterpret_cast<uint2 *>(a.q8 + row * a.D + i) = make_uint2(w[0], w[1]);
-            else a.q8[row * a.D + i] = (int8_t)w[0];
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(part.y)));
         }
-        if (a.y) {
-            float y[N];
+        const float inv = rsqrtf(__fdiv_rn(sum, (float)a.D) + a.eps);
+        // below 127 / FLT_MAX the factor would be infinite: such a row counts as zero
+        const bool zero = !(top > 3.8e-37f);
+        const float to8 = zero ? 0.0f : __fmul_rn(__frcp_rn(top), 127.0f);
 #pragma unroll
-            for (int k = 0; k < N; k++) y[k] = r[p][k] * inv;
-            store_n(a.y + row * a.D + i, y);
+        for (int p = 0; p < P; p++) {
+            if (place(p) >= a.D) break;
+            if (a.q8) {
+                // x + 1.5 2^23 rounds x to a whole number, half to even, whose low byte is the int8
+                uint32_t w[N];
+#pragma unroll
+                for (int k = 0; k < N; k++) w[k] = __float_as_uint(__fadd_rn(__fmul_rn(r[p][k], to8), 12582912.0f));
+                int8_t *q = a.q8 + row * a.D + place(p);
+                if constexpr (N == 8)
+                    *reinterpret_cast<uint2 *>(q) =
+                        make_uint2(__byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410),
+                                   __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410));
+                else
+                    *q = (int8_t)w[0];
+            }
+            if (a.y) {
+                float y[N];
+#pragma unroll
+                for (int k = 0; k < N; k++) y[k] = r[p][k] * inv;
+                store_n(a.y + row * a.D + place(p), y);
+            }
         }
+        if (a.scale && threadIdx.x == 0) a.scale[row] = zero ? 1.0f : __fmul_rn(__fdiv_rn(top, 127.0f), inv);
     }
-    if (a.scale && threadIdx.x == 0) a.scale[row] = zero ? 1.0f : __fmul_rn(__fdiv_rn(top, 127.0f), inv);
 }
 
-// threads and pieces: enough threads that a thread keeps one piece, up to 256 of them; then up to 4
-// pieces of 8 (16 of 1), which 512 (1024) threads cover D = 16384 with
-template <typename X, typename R>
-cudaError_t launch_norm(const NormArgs &a, int M, bool wide, cudaStream_t st) {
-    const int pieces = wide ? a.D / 8 : a.D;
-    auto threads = [&](int p) { return std::max(32, ((pieces + p - 1) / p + 31) / 32 * 32); };
-    if (wide) {
-        if (pieces <= 256) rmsnorm_kernel<X, R, 8, 1><<<M, threads(1), 0, st>>>(a);
-        else if (pieces <= 512) rmsnorm_kernel<X, R, 8, 2><<<M, threads(2), 0, st>>>(a);
-        else rmsnorm_kernel<X, R, 8, 4><<<M, threads(4), 0, st>>>(a);
-    } else {
-        if (pieces <= 1024) rmsnorm_kernel<X, R, 1, 4><<<M, threads(4), 0, st>>>(a);
-        else rmsnorm_kernel<X, R, 1, 16><<<M, threads(16), 0, st>>>(a);
-    }
+template <typename X, typename R, int N, int P, int kThreads, bool kAhead>
+cudaError_t launch_norm(const NormArgs &a, int sms, cudaStream_t st) {
+    const int pieces = (a.D + N - 1) / N, threads = std::max(32, ((pieces + P - 1) / P + 31) / 32 * 32);
+    // as many CTAs as fit (64 to 80 registers a thread), and a row more to each
+    const int64_t grid = kAhead ? std::min<int64_t>(a.M, (int64_t)sms * std::max(1, std::min(16, 768 / threads))) : a.M;
+    rmsnorm_kernel<X, R, N, P, kThreads, kAhead><<<(unsigned)grid, threads, 0, st>>>(a);
     return cudaGetLastError();
+}
+template <typename X, typename R>
+cudaError_t launch_norm(const NormArgs &a, bool wide, int sms, cudaStream_t st) {
+    if (wide) {
+        if (a.D <= 2048) return launch_norm<X, R, 8, 1, 256, true>(a, sms, st);
+        if (a.D <= 4096) return launch_norm<X, R, 8, 2, 256, true>(a, sms, st);
+        return launch_norm<X, R, 8, 2, 1024, false>(a, sms, st);
+    }
+    if (a.D <= 1024) return launch_norm<X, R, 1, 4, 256, true>(a, sms, st);
+    if (a.D <= 4096) return launch_norm<X, R, 1, 4, 1024, false>(a, sms, st);
+    return launch_norm<X, R, 1, 16, 1024, false>(a, sms, st);
 }
 
 // ---------------------------------------------------------------------------------- logits
@@ -545,17 +583,21 @@ int xdna_rmsnorm_residual_i8(const void *x, int x_f32, int64_t x_stride, const v
     if (x_stride < D || ((residual || residual_out) && res_stride < D)) return fail(me + "a row stride below D");
     if (!(eps >= 0.0f)) return fail(me + "negative eps");
     if (M == 0) return 0;
-    NormArgs a{x, residual, x_stride, res_stride, gamma, unit_offset, D, eps, residual_out,
+    NormArgs a{x, residual, x_stride, res_stride, gamma, unit_offset, M, D, eps, residual_out,
                reinterpret_cast<__nv_bfloat16 *>(y_bf16), q8, scale};
     auto st = static_cast<cudaStream_t>(stream);
+    int dev = 0, sms = 0;
+    if (!ck(cudaGetDevice(&dev), "xdna_rmsnorm_residual_i8") ||
+        !ck(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "xdna_rmsnorm_residual_i8"))
+        return -1;
     const int xe = x_f32 ? 4 : 8, re = res_f32 ? 4 : 8;    // elements of 16 bytes
     const bool wide = D % 8 == 0 && x_stride % xe == 0 && (!(residual || residual_out) || res_stride % re == 0) &&
                       aligned16(x) && aligned16(gamma) && aligned16(residual) && aligned16(residual_out) && aligned16(y_bf16) &&
                       reinterpret_cast<uintptr_t>(q8) % 8 == 0;
-    const cudaError_t e = x_f32 ? (res_f32 ? launch_norm<float, float>(a, M, wide, st)
-                                           : launch_norm<float, __nv_bfloat16>(a, M, wide, st))
-                                : (res_f32 ? launch_norm<__nv_bfloat16, float>(a, M, wide, st)
-                                           : launch_norm<__nv_bfloat16, __nv_bfloat16>(a, M, wide, st));
+    const cudaError_t e = x_f32 ? (res_f32 ? launch_norm<float, float>(a, wide, sms, st)
+                                           : launch_norm<float, __nv_bfloat16>(a, wide, sms, st))
+                                : (res_f32 ? launch_norm<__nv_bfloat16, float>(a, wide, sms, st)
+                                           : launch_norm<__nv_bfloat16, __nv_bfloat16>(a, wide, sms, st));
     return ck(e, "xdna_rmsnorm_residual_i8") ? 0 : -1;
 }
 

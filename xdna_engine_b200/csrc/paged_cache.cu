@@ -79,18 +79,24 @@ struct AppendArgs {
     int64_t q_stride, k_stride, v_stride;
     const int32_t *seq, *pos;
     const float *rope;
-    int n_tokens, n_q_heads, rope_rows, rot, interleaved;
+    int n_tokens, n_q_heads, rope_rows, rot, interleaved, page_shift;
     __nv_bfloat16 *q_out;
     unsigned *status;
 };
 
+// values that are read once pass L1 by, which holds the rotary rows that all heads of a token read
+__device__ __forceinline__ void load8_rope(const float *p, float (&x)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
 __device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+    const float4 a = __ldcs(reinterpret_cast<const float4 *>(p)), b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
 }
 __device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&x)[8]) {
-    const uint4 a = *reinterpret_cast<const uint4 *>(p);
+    const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(p));
     const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -101,30 +107,33 @@ __device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&x)[8]) {
 __device__ __forceinline__ void store8(__nv_bfloat16 *p, const float (&x)[8]) {
     uint32_t u[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) u[i] = xdna::bf16bits(x[2 * i]) | (xdna::bf16bits(x[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; i++) {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        u[i] = *reinterpret_cast<const uint32_t *>(&two);
+    }
     *reinterpret_cast<uint4 *>(p) = make_uint4(u[0], u[1], u[2], u[3]);
 }
-__device__ __forceinline__ uint32_t whole8(float x, float inv) {
-    return (uint32_t)(max(-127, min(127, __float2int_rn(__fmul_rn(x, inv))))) & 0xffu;
-}
+// x inv + 1.5 2^23 rounds x inv to a whole number, half to even, whose low byte is the int8
 __device__ __forceinline__ void store8(int8_t *p, const float (&x)[8], float inv) {
-    uint32_t u[2] = {0, 0};
+    uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) u[i / 4] |= whole8(x[i], inv) << (8 * (i % 4));
-    *reinterpret_cast<uint2 *>(p) = make_uint2(u[0], u[1]);
+    for (int i = 0; i < 8; i++) w[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.0f));
+    *reinterpret_cast<uint2 *>(p) =
+        make_uint2(__byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410),
+                   __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410));
 }
 
 // One lane per 16 components of a row (a token's head): the two 8-component chunks whose pairs turn
 // together, so that a lane holds both halves of its pairs; a row's D / 16 lanes lie side by side in
 // a warp, which gives the int8 row's maximum by shuffles.
 template <int D, typename Src, bool I8>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, 6) append_kernel(const AppendArgs a) {
     constexpr int L = D / 16;
     const int heads = (a.q ? a.n_q_heads : 0) + 2 * a.pool.n_kv_heads, first_k = heads - 2 * a.pool.n_kv_heads;
-    const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / L;
+    const unsigned item = blockIdx.x * (256 / L) + threadIdx.x / L;   // n_tokens * heads are below 2^31
     const int lane = threadIdx.x % L;
-    const bool live = item < (int64_t)a.n_tokens * heads;
-    const int t = live ? (int)(item / heads) : 0, hh = live ? (int)(item % heads) : 0;
+    const bool live = item < (unsigned)a.n_tokens * heads;
+    const int t = live ? item / heads : 0, hh = live ? item - t * heads : 0;
     const int kind = hh < first_k ? 0 : hh < first_k + a.pool.n_kv_heads ? 1 : 2;
     const int h = kind == 0 ? hh : (hh - first_k) % a.pool.n_kv_heads;
 
@@ -136,8 +145,8 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
         if (a.rope && pos >= a.rope_rows) bad |= kBadPosition;
         if (kind) {
             const int s = a.seq ? a.seq[t] : t;
-            const int col = pos / a.pool.page_size;
-            slot = pos % a.pool.page_size;
+            const int col = a.page_shift >= 0 ? pos >> a.page_shift : pos / a.pool.page_size;
+            slot = pos - col * a.pool.page_size;
             if (s < 0 || s >= a.table.n_seqs) bad |= kBadStream;
             else if (col >= a.table.width) bad |= kBadPosition;
             else {
@@ -165,8 +174,8 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
         if (turned) {
             const float *r = a.rope + (int64_t)pos * a.rot + 8 * lane;
             float cs[8], sn[8];
-            load8(r, cs);
-            load8(r + a.rot / 2, sn);
+            load8_rope(r, cs);
+            load8_rope(r + a.rot / 2, sn);
             auto turn = [](float &u, float &w, float c, float s) {
                 const float p = __fsub_rn(__fmul_rn(u, c), __fmul_rn(w, s));
                 w = __fadd_rn(__fmul_rn(w, c), __fmul_rn(u, s));
@@ -1073,6 +1082,9 @@ Pool pool_of(const XdnaPagedCache *c, int layer) {
     return p;
 }
 
+// log2 of a page size that is a power of two, else -1
+int shift_of(int page_size) { return page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size); }
+
 // NULL, or what is wrong with a call's block table
 const char *table_fault(const int32_t *table, int n_seqs, int width, int64_t stride) {
     if (!table) return "null block table";
@@ -1196,9 +1208,10 @@ int xdna_paged_append(XdnaPagedCache *c, int layer, int n_tokens, int n_q_heads,
     a.n_tokens = n_tokens; a.n_q_heads = q ? n_q_heads : 0;
     a.q_out = reinterpret_cast<__nv_bfloat16 *>(q_out);
     a.status = c->status;
-    const int64_t lanes = (int64_t)n_tokens * (a.n_q_heads + 2 * g.n_kv_heads) * (g.head_dim / 16);
-    const int64_t blocks = (lanes + 255) / 256;
-    if (blocks > 0x7fffffff) return fail(me + "too many tokens for one call");
+    a.page_shift = shift_of(g.page_size);
+    const int64_t rows = (int64_t)n_tokens * (a.n_q_heads + 2 * g.n_kv_heads), at_once = 4096 / g.head_dim;
+    if (rows > 0x7fff0000) return fail(me + "more than 2^31 rows in one call");
+    const int64_t blocks = (rows + at_once - 1) / at_once;
     auto st = static_cast<cudaStream_t>(stream);
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
@@ -1247,7 +1260,7 @@ int xdna_paged_attention(XdnaPagedCache *c, int layer, const uint16_t *q, int64_
     a.lse = lse;
     a.status = c->status;
     a.group = n_q_heads / g.n_kv_heads;
-    a.page_shift = g.page_size & (g.page_size - 1) ? -1 : __builtin_ctz(g.page_size);
+    a.page_shift = shift_of(g.page_size);
     a.whole_steps = g.page_size % kStep == 0;
     a.dense_steps = a.whole_steps && g.stride_slot == g.head_dim;
     a.part_o = c->part_o;
