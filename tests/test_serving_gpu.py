@@ -258,6 +258,12 @@ def test_attention_bad_pages_are_reported(X, dev):
             c.check()
         check_attention(out[1:], None, tuple(w[1:] for w in want))
         assert torch.isfinite(out.float()).all()
+    lse = torch.empty(2, 4, device="cuda")
+    out = c.attend(q, torch.stack([torch.full_like(p["table"][0], -3), p["table"][1]]), t, lse=lse)
+    with pytest.raises(X.XdnaError, match="page id"):
+        c.check()
+    assert not out[0].any() and bool((lse[0] == -math.inf).all())          # nothing left: zeros
+    check_attention(out[1:], lse[1:], tuple(w[1:] for w in want))
     out = c.attend(q, p["table"], torch.tensor([100, 113], dtype=I32, device="cuda"))
     with pytest.raises(X.XdnaError, match="position"):
         c.check()
@@ -366,6 +372,18 @@ def test_append(X, dev, hq, hkv, d, rot, interleaved, src, kv):
         old[1, pg, :, at] = pool[1, pg, :, at]
         assert torch.equal(pool.view(torch.int16 if kv == "bf16" else I8),
                            old.view(torch.int16 if kv == "bf16" else I8))          # nothing else was written
+
+
+def test_append_one_token_of_any_stride(X, dev):
+    """A single token's strides say nothing: x[None] of a transposed product is taken."""
+    g = rng(12)
+    pool = torch.zeros(2, 2, 16, 64, dtype=BF16, device="cuda")
+    c = X.PagedCache(dev, pool, pool.clone())
+    k = torch.randn(2, 64, generator=g, device="cuda").to(BF16)
+    odd = k.as_strided((1, 2, 64), (1, 64, 1))
+    c.append(odd, odd, odd, None, torch.tensor([3], dtype=I32, device="cuda"), torch.tensor([[1]], dtype=I32, device="cuda"))
+    c.check()
+    assert torch.equal(pool[1, :, 3], k) and int((pool != 0).any(-1).sum()) == 2
 
 
 def test_append_bad_inputs_are_reported(X, dev):

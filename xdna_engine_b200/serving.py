@@ -78,7 +78,7 @@ def _heads(x, dtype, n, d, dev, name):
             or (s[1] != d and shape[1] != 1) or x.get_device() != dev):
         raise ValueError(f"{name}: want {dtype} [{n}, heads, {d}] with contiguous heads on GPU {dev}, got {x.dtype} "
                          f"{tuple(shape)} on {x.device}, strides {s}")
-    return shape[1], s[0]
+    return shape[1], s[0] if n > 1 else shape[1] * d
 
 
 def _table(t, dev):
@@ -195,7 +195,7 @@ class PagedCache:
         if n == 0:
             return out
         if (_L or _lib()).xdna_paged_attention(
-                self.handle, layer, q.data_ptr(), qs if n > 1 else hq * d, hq, block_table.data_ptr(), n, width, ts,
+                self.handle, layer, q.data_ptr(), qs, hq, block_table.data_ptr(), n, width, ts,
                 _flat(seq_lens, torch.int32, n, dev, "seq_lens"), d ** -0.5 if scale is None else scale, window,
                 _flat(out, torch.bfloat16, n * hq * d, dev, "out"), _flat(lse, torch.float32, n * hq, dev, "lse"),
                 _raw_stream(dev) if stream is None else stream):
