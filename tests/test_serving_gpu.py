@@ -537,6 +537,26 @@ def test_logits(X, b, v, src, what):
         assert out2 is x and torch.equal(x, out) and torch.equal(got, got2)
 
 
+@pytest.mark.parametrize("src", [F32, BF16])
+@pytest.mark.parametrize("b,v", [(40, 70001), (20, 100000)])
+def test_logits_long_histories(X, b, v, src):
+    """Many long rows (their histories are sorted by chunk first), one of them empty, one of a single token."""
+    r = np.random.default_rng(b)
+    x = torch.from_numpy((r.standard_normal((b, v)) * 3).astype(np.float32)).cuda().to(src)
+    hist = [(v * r.random(n) ** 3).astype(np.int32) for n in r.integers(0, 12000, b)]
+    hist[3], hist[4] = hist[3][:0], np.full(9000, v - 1, np.int32)
+    hist[5] = np.concatenate([hist[5], np.array([-1, v, 2**31 - 1, -2**31, 0, 0], np.int32)])
+    npr = np.array([r.integers(0, len(h) + 1) for h in hist], np.int32)
+    rep, freq, pres = ((r.random(b) + 0.6).astype(np.float32) for _ in range(3))
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    want, ids = logits_plain(x.float().cpu().numpy(), hist, npr, rep, freq, pres, None, None)
+    out, got = X.process_logits(x, history=dev(np.concatenate(hist)),
+                                history_start=dev(np.cumsum([0] + [len(h) for h in hist]).astype(np.int32)),
+                                n_prompt=dev(npr), repetition=dev(rep), frequency=dev(freq), presence=dev(pres))
+    assert np.array_equal(out.cpu().numpy().view(np.uint32), want.view(np.uint32))
+    assert np.array_equal(got.cpu().numpy(), ids)
+
+
 def test_logits_ties_and_odd_values(X):
     """Equal maxima go to the lowest id, across the whole row; NaN is never chosen and a masked NaN or
     infinity becomes -inf; +inf wins; -0 and 0 are equal."""

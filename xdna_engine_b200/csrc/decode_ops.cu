@@ -320,6 +320,19 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const LogitsA
     const T *x = static_cast<const T *>(a.logits) + b * a.stride + first;
     float *out = a.out + b * a.out_stride + first;
     auto place_of = [&](int p) { return (p * kLogitsThreads + tid) * W; };
+    const bool lists = a.hist || a.bias;
+    int h0 = 0, h1 = 0, gen = 0, e0 = 0, e1 = 0;
+    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    if (lists) {                                          // the lists' ids wait for these: first of all
+        h0 = a.hist ? a.hist_start[b] : 0;
+        h1 = a.hist ? a.hist_start[b + 1] : 0;
+        gen = a.n_prompt ? a.n_prompt[b] : 0;
+        e0 = a.bias ? a.bias_start[b] : 0;
+        e1 = a.bias ? a.bias_start[b + 1] : 0;
+        rep = a.rep ? a.rep[b] : 1.0f;
+        freq = a.freq ? a.freq[b] : 0.0f;
+        pres = a.pres ? a.pres[b] : 0.0f;
+    }
     float y[P][W];
     unsigned allowed = 0xffffffffu;                       // bit p W + w
     const uint32_t *mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
@@ -335,10 +348,11 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const LogitsA
                 y[p][w] = i >= lo && i < hi ? to_f32(x[i]) : -INFINITY;
             }
     }
-    if (mask && full && shift == 0) {
-        allowed = 0;
+    const bool whole_words = mask && full && shift == 0;
+    unsigned word[P];
+    if (whole_words) {
 #pragma unroll
-        for (int p = 0; p < P; p++) allowed |= ((mask[(first + place_of(p)) / 32] >> (place_of(p) % 32)) & kPiece) << (p * W);
+        for (int p = 0; p < P; p++) word[p] = mask[(first + place_of(p)) / 32];
     } else if (mask) {
         allowed = 0;
 #pragma unroll
@@ -349,12 +363,12 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const LogitsA
                 if (i >= lo && i < hi) allowed |= ((mask[(first + i) / 32] >> ((first + i) % 32)) & 1u) << (p * W + w);
             }
     }
-    const bool lists = a.hist || a.bias;
     if (lists) {
-        const int h0 = a.hist ? max(0, a.hist_start[b]) : 0, h1 = a.hist ? min(a.n_hist, a.hist_start[b + 1]) : 0;
-        const int gen = a.n_prompt ? min(max(0, a.n_prompt[b]), 0x7fffffff - h0) + h0 : h0;
-        const int e0 = a.bias ? max(0, a.bias_start[b]) : 0, e1 = a.bias ? min(a.n_bias, a.bias_start[b + 1]) : 0;
-        const float rep = a.rep ? a.rep[b] : 1.0f, freq = a.freq ? a.freq[b] : 0.0f, pres = a.pres ? a.pres[b] : 0.0f;
+        h0 = max(0, h0);
+        h1 = min(a.n_hist, h1);
+        gen = min(max(0, gen), 0x7fffffff - h0) + h0;
+        e0 = max(0, e0);
+        e1 = min(a.n_bias, e1);
         int biased = e1 - e0 > tid ? a.bias_ids[e0 + tid] : -1;
         int ids[kAhead];
         auto ahead = [&](int j0) {
@@ -412,6 +426,11 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const LogitsA
         __syncthreads();
     }
     // ---- every id
+    if (whole_words) {
+        allowed = 0;
+#pragma unroll
+        for (int p = 0; p < P; p++) allowed |= ((word[p] >> (place_of(p) % 32)) & kPiece) << (p * W);
+    }
     float top = -INFINITY;
 #pragma unroll
     for (int p = 0; p < P; p++) {
