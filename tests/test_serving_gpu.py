@@ -218,6 +218,31 @@ def test_attention_negative_and_spiked(X, dev):
     assert torch.isnan(out[1].float()).all() and torch.isfinite(out[0].float()).all()
 
 
+def test_int8_rows_keep_a_nan(X, dev):
+    """A NaN in an appended row, or a NaN scale of a live key or value, shows in the result; in the rows
+    past a stream's length it does not."""
+    g = rng(13)
+    pools = [torch.zeros(4, 1, 16, 64, dtype=I8, device="cuda") for _ in "kv"]
+    scales = [torch.full((4, 1, 16), math.nan, device="cuda") for _ in "kv"]
+    c = X.PagedCache(dev, *pools, *scales)
+    table = torch.tensor([[0], [1]], dtype=I32, device="cuda")
+    pos = torch.arange(8, dtype=I32, device="cuda")
+    for stream in (0, 1):
+        k, v = (torch.randn(8, 1, 64, generator=g, device="cuda") for _ in "kv")
+        if stream:
+            v[5, 0, 7] = math.nan
+        c.append(None, k, v, torch.full_like(pos, stream), pos, table)
+    q = torch.randn(2, 4, 64, generator=g, device="cuda").to(BF16)
+    out = c.attend(q, table, torch.tensor([8, 8], dtype=I32, device="cuda")).float()
+    assert torch.isfinite(out[0]).all() and torch.isnan(out[1]).all()
+    out = c.attend(q, table, torch.tensor([8, 5], dtype=I32, device="cuda")).float()
+    assert torch.isfinite(out).all()
+    scales[0][0, 0, 3] = math.nan
+    out = c.attend(q, table, torch.tensor([8, 5], dtype=I32, device="cuda")).float()
+    assert torch.isnan(out[0]).all() and torch.isfinite(out[1]).all()
+    c.check()
+
+
 def test_attention_past_32_bits(X, dev):
     """Pages whose elements lie past 2^31 in the pool."""
     g = rng(7)

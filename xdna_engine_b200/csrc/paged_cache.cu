@@ -125,7 +125,10 @@ __device__ __forceinline__ void store8(int8_t *p, const float (&x)[8], float inv
 
 // One lane per 16 components of a row (a token's head): the two 8-component chunks whose pairs turn
 // together, so that a lane holds both halves of its pairs; a row's D / 16 lanes lie side by side in
-// a warp, which gives the int8 row's maximum by shuffles.
+// a warp, which gives the int8 row's maximum by shuffles.  4 or 2 bytes in and 2 or 1 out per element, so
+// HBM bounds it; a token's rotary row comes from L1 for all its heads but the first.  Measured: 8192 tokens
+// of 32/8 heads x 128, f32 in, 52.5 us (5.8 TB/s; several heads to a lane, with the rotary row kept in
+// registers: 60 us); 2003 tokens of 4/1 x 256 into int8 5.0 us; 64 tokens 2.5 us.
 template <int D, typename Src, bool I8>
 __global__ void __launch_bounds__(256, 6) append_kernel(const AppendArgs a) {
     constexpr int L = D / 16;
@@ -201,14 +204,16 @@ __global__ void __launch_bounds__(256, 6) append_kernel(const AppendArgs a) {
         if (!I8) return;                   // int8: the row's lanes all reach the shuffles below
     }
     if constexpr (I8) {
-        float top = 0.0f;
+        // magnitudes ordered as bits, so that a NaN is the largest and makes the row's scale NaN
+        unsigned bits = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) top = fmaxf(top, fmaxf(fabsf(x[i]), fabsf(y[i])));
+        for (int i = 0; i < 8; i++) bits = max(bits, max(__float_as_uint(fabsf(x[i])), __float_as_uint(fabsf(y[i]))));
 #pragma unroll
-        for (int o = 1; o < L; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = 1; o < L; o *= 2) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
         if (kind == 0 || !live || skip) return;
+        const float top = __uint_as_float(bits);
         // below 127 / FLT_MAX the factor would be infinite: such a row counts as zero
-        const bool zero = !(top > 3.8e-37f);
+        const bool zero = top <= 3.8e-37f;
         const float inv = zero ? 0.0f : __fmul_rn(__frcp_rn(top), 127.0f);
         const int64_t row = ((int64_t)page * a.pool.n_kv_heads + h) * a.pool.page_size + slot;
         int8_t *o = static_cast<int8_t *>(kind == 1 ? a.pool.k : a.pool.v) + page * a.pool.sp + h * a.pool.sh +
@@ -256,6 +261,10 @@ __global__ void __launch_bounds__(256, 6) append_kernel(const AppendArgs a) {
 // HBM as the bound.  q is scaled there by a power of two per head to fp16's upper range; a
 // value's scale v_scale goes into the exponent, w_j = exp2(s_j + log2 v_scale_j - max + 14), which fp16
 // holds whatever the scales.
+//
+// Measured: 64 streams of 0 to 8k, 32/8 heads x 128, pages of 16, 183 us (5.9 TB/s, 90 % of a copy); 4 x 64k
+// in int8 101 us (5.5 TB/s; issue-bound next); 32 streams of 0 to 2k, 12 heads x 64, 27.5 us; one stream
+// of 4k, 4/1 x 256, 13.2 us, a chain of waits.
 constexpr int kWarps = 4, kStep = 16, kTileKeys = kWarps * kStep;
 
 struct AttnArgs {
@@ -444,10 +453,12 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
         empty_streams();
         return;
     }
-    // Short units, one CTA to each: what is left then to join within it takes less than parts would.  Else no
+    // Short units, one CTA to each: its own steps take less than a join would (32 streams x 5 heads of 3
+    // tiles 7.5 us, in parts 9.8; 6 x 3 of up to 10 tiles 12.6 us, in parts 9.0).  Else no
     // share is empty, so that a unit's parts lie in consecutive CTAs (one may hold an end alone): up to 64
-    // tiles a unit, no more CTAs than make 16 parts of the longest; units of one length and few tiles,
-    // as many CTAs to each, whose parts then all have an end
+    // tiles a unit, no more CTAs than make 16 parts of the longest (one unit of 64 tiles: 13.2 us, 8 parts
+    // 18.3, 32 parts 13.5); units of one length and few tiles, as many CTAs to each, whose parts then
+    // all have an end (64 units of 8 tiles: 14.2 us, else 19.0)
     const bool apart = live_units <= (Int)gridDim.x && longest <= S::kApartTiles;
     Int want = min((Int)gridDim.x, total);
     if (longest <= 4 * kJoinWays) want = min(want, total * kJoinWays / longest);
@@ -738,8 +749,8 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
                 if constexpr (I8) {
                     const float *sc = reinterpret_cast<const float *>(tail);
                     f0 = sc[g]; f1 = sc[g + 8];
-                    v0 = log2_approx(fmaxf(sc[16 + g], 1e-30f));
-                    v1 = log2_approx(fmaxf(sc[24 + g], 1e-30f));
+                    v0 = log2_approx(sc[16 + g] < 1e-30f ? 1e-30f : sc[16 + g]);   // a NaN stays one
+                    v1 = log2_approx(sc[24 + g] < 1e-30f ? 1e-30f : sc[24 + g]);
                 }
                 float den[NT][4];                         // the exponents of the sum's terms, s[.][0] the weights'
                 bool up = false;
@@ -1058,6 +1069,7 @@ cudaError_t launch_attention(AttnArgs a, int sms, cudaStream_t st) {
 }
 template <int D>
 cudaError_t launch_attention(const AttnArgs &a, bool i8, int sms, cudaStream_t st) {
+    // up to 16 heads to a unit: 32 x 8k, 64/4 heads x 128 takes 103 us, as two units of 8 that read K and V twice 176
     if (a.group <= 8) return i8 ? launch_attention<D, true, 1>(a, sms, st) : launch_attention<D, false, 1>(a, sms, st);
     return i8 ? launch_attention<D, true, 2>(a, sms, st) : launch_attention<D, false, 2>(a, sms, st);
 }
