@@ -574,7 +574,7 @@ int xdna_paged_append(XdnaPagedCache *c, int layer, int n_tokens, int n_q_heads,
  * q bf16, streams q_stride elements apart; query head h reads K/V head h / (n_q_heads /
  * n_kv_heads).  Scores, softmax and sums in f32, the weights to 16 bits of mantissa.  A stream
  * of no positions (seq_lens <= 0), or whose every score is -inf, gives zeros.  lse (NULL: none) [n_seqs][n_q_heads] f32: the
- * log of the sum of exponentials, -inf for no positions. */
+ * log of the sum of exponentials, -inf for no positions.  out may not overlap q. */
 int xdna_paged_attention(XdnaPagedCache *c, int layer, const uint16_t *q, int64_t q_stride, int n_q_heads,
                          const int32_t *block_table, int n_seqs, int table_width, int64_t table_stride,
                          const int32_t *seq_lens, float scale, int window, uint16_t *out, float *lse, void *stream);

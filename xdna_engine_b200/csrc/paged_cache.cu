@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(256, 6) append_kernel(const AppendArgs a) {
 //
 // Measured: 64 streams of 0 to 8k, 32/8 heads x 128, pages of 16, 183 us (5.9 TB/s, 90 % of a copy); 4 x 64k
 // in int8 101 us (5.5 TB/s; issue-bound next); 32 streams of 0 to 2k, 12 heads x 64, 27.5 us; one stream
-// of 4k, 4/1 x 256, 13.2 us, a chain of waits.
+// of 4k, 4/1 x 256, 12.4 us, a chain of waits.
 constexpr int kWarps = 4, kStep = 16, kTileKeys = kWarps * kStep;
 
 struct AttnArgs {
@@ -288,19 +288,26 @@ constexpr int kJoinWays = 16, kJoinLevels = 3;            // 16^3 parts
 
 template <int D, bool I8, int NT>
 struct AttnShape {
-    static constexpr int kRowBytes = D * (I8 ? 1 : 2);
+    // bf16 rows of 256 are halved between two warps, which both work on a step's 16 keys and exchange their parts
+    // of the scores: one CTA's ring fills the SM, and 4 warps are one to a scheduler (one stream of 4k
+    // 13.1 us so, 12.4 us with pairs; 53 streams to 5.8k 39.8 and 37.3 us)
+    static constexpr int kPair = D == 256 && !I8 ? 2 : 1, kPart = D / kPair;   // components to a warp
+    static constexpr int kThreads = 32 * kWarps * kPair;
+    static constexpr int kRowBytes = kPart * (I8 ? 1 : 2);
     static constexpr int kRows = 2 * kStep * kRowBytes;                  // K and V of a step
     static constexpr int kStages = kRows >= 8192 ? 3 : kRows >= 4096 ? 4 : 6;
     static constexpr int kStage = kRows + (I8 ? 128 : 0) + 16;           // + scales, + live mask
     static constexpr int kHeads = 8 * NT;
     static constexpr int kEndCost = 2, kApartTiles = 4;
-    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kRing = kWarps * kPair * kStages * kStage;
     static constexpr int kJoinCols = 32, kJoinRow = kJoinCols + 4;
-    static constexpr int kJoin = kWarps * kHeads * kJoinRow * 4;
+    static constexpr int kJoin = kWarps * kPair * kHeads * kJoinRow * 4;
+    static_assert(kPair == 1 || kJoin >= 2 * kWarps * kPair * 32 * NT * 16, "a pair's scores, twice, lie there too");
     static constexpr int kQRow = D + 8;
     static constexpr int kQ = kHeads * kQRow * 2 + kHeads * 4;           // q, and an int8 pool's factors
-    static constexpr bool kQInRegs = !(D == 256 && NT == 2);             // 64 registers of q beside 128 of o would spill
+    static constexpr bool kQInRegs = !(kPart == 256 && NT == 2);             // 64 registers of q beside 128 of o would spill
     static constexpr int kSmem = kRing + kJoin + kQ;
+    static_assert(kSmem + 2048 <= 227 * 1024, "shared memory");
     static constexpr int kCtas = 3 * (kSmem + 1800) <= 228 * 1024 ? 3 : 2 * (kSmem + 1800) <= 228 * 1024 ? 2 : 1;
 };
 
@@ -386,20 +393,23 @@ __device__ __forceinline__ Live live_keys(const AttnArgs &a, int n) {
 }
 
 template <int D, bool I8, int NT, bool kSmall>
-__global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D, I8, NT>::kCtas)) attention_kernel(const AttnArgs a) {
     using S = AttnShape<D, I8, NT>;
     constexpr int kChunks = S::kRowBytes / 16, kRowsPerCopy = kChunks >= 32 ? 1 : 32 / kChunks, kCopies = kStep / kRowsPerCopy;
-    constexpr int kMt = D / 16, kElem = I8 ? 1 : 2;
+    constexpr int kMt = S::kPart / 16, kElem = I8 ? 1 : 2, kThreads = S::kThreads;
     constexpr float kLift = I8 ? 14.0f : 0.0f;            // weights reach up to 2^kLift
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float join_m[kWarps][S::kHeads], join_l[kWarps][S::kHeads];
     __shared__ int last;
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, j = lane % 4;
-    unsigned char *ring = smem + warp * S::kStages * S::kStage;
+    // warp: which 16 keys of a tile; half: which of a pair's two
+    const int tid = threadIdx.x, any_warp = tid / 32, warp = any_warp / S::kPair, half = any_warp % S::kPair;
+    const int lane = tid % 32, g = lane / 4, j = lane % 4;
+    unsigned char *ring = smem + any_warp * S::kStages * S::kStage;
     const uint32_t ring_u = xdna::smem_u32(ring);
     float *join_o = reinterpret_cast<float *>(smem + S::kRing);
     uint16_t *q_s = reinterpret_cast<uint16_t *>(smem + S::kRing + S::kJoin);
     float *q_inv = reinterpret_cast<float *>(q_s + S::kHeads * S::kQRow);
+    [[maybe_unused]] float *swap = reinterpret_cast<float *>(smem + S::kRing);   // pairs' scores, between joins
     // ---- streams of no keys, once the CTA is through
     auto empty_streams = [&]() {
         for (int b = blockIdx.x; b < a.table.n_seqs; b += gridDim.x) {
@@ -407,9 +417,9 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
             if (n > a.table.width * a.pool.page_size && tid == 0) atomicOr(a.status, kBadPosition);
             if (n > 0) continue;
             uint4 *out = reinterpret_cast<uint4 *>(a.out + (int64_t)b * a.n_q_heads * D);
-            for (int i = tid; i < a.n_q_heads * (D / 8); i += 128) out[i] = make_uint4(0, 0, 0, 0);
+            for (int i = tid; i < a.n_q_heads * (D / 8); i += kThreads) out[i] = make_uint4(0, 0, 0, 0);
             if (a.lse)
-                for (int i = tid; i < a.n_q_heads; i += 128) a.lse[(int64_t)b * a.n_q_heads + i] = -INFINITY;
+                for (int i = tid; i < a.n_q_heads; i += kThreads) a.lse[(int64_t)b * a.n_q_heads + i] = -INFINITY;
         }
     };
 
@@ -456,9 +466,9 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
     // Short units, one CTA to each: its own steps take less than a join would (32 streams x 5 heads of 3
     // tiles 7.5 us, in parts 9.8; 6 x 3 of up to 10 tiles 12.6 us, in parts 9.0).  Else no
     // share is empty, so that a unit's parts lie in consecutive CTAs (one may hold an end alone): up to 64
-    // tiles a unit, no more CTAs than make 16 parts of the longest (one unit of 64 tiles: 13.2 us, 8 parts
-    // 18.3, 32 parts 13.5); units of one length and few tiles, as many CTAs to each, whose parts then
-    // all have an end (64 units of 8 tiles: 14.2 us, else 19.0)
+    // tiles a unit, no more CTAs than make 16 parts of the longest (one unit of 64 tiles: 13.2 us, in 8 parts
+    // 18.3, in 32 13.5); units of one length and few tiles, as many CTAs to each, whose parts then
+    // all have an end (64 units of 8 tiles: 14.3 us, else 19.0)
     const bool apart = live_units <= (Int)gridDim.x && longest <= S::kApartTiles;
     Int want = min((Int)gridDim.x, total);
     if (longest <= 4 * kJoinWays) want = min(want, total * kJoinWays / longest);
@@ -556,17 +566,17 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
         if (unfetched <= 0) return;
         const uint32_t base = ring_u + stage * S::kStage;
         const int pos = ahead.live.first + (ahead.t * kWarps + warp) * kStep;
-        const unsigned char *kb = static_cast<const unsigned char *>(a.pool.k) + ahead_hk * a.pool.sh * kElem;
+        const unsigned char *kb = static_cast<const unsigned char *>(a.pool.k) + ahead_hk * a.pool.sh * kElem + half * S::kRowBytes;
         unsigned mask = 0xffffu;
         if (a.dense_steps && pos >= ahead.live.x && pos + kStep <= ahead.live.y && (unsigned)page < (unsigned)a.pool.n_pages) {
             // 16 whole rows side by side
             const int slot = a.page_shift >= 0 ? pos & ((1 << a.page_shift) - 1) : pos % a.pool.page_size;
-            const unsigned char *at = kb + page * a.pool.sp * kElem + slot * S::kRowBytes + lane * 16;
+            const unsigned char *at = kb + page * a.pool.sp * kElem + (slot + lane_row) * (D * kElem) + lane_chunk * 16;
 #pragma unroll
             for (int i = 0; i < kCopies; i++) {
                 const uint32_t dst = base + swizzled(i * kRowsPerCopy + lane_row, lane_chunk);
-                cp_async16_or_zero(dst, at + i * 512, true);
-                cp_async16_or_zero(dst + kStep * S::kRowBytes, at + kv + i * 512, true);
+                cp_async16_or_zero(dst, at + i * kRowsPerCopy * D * kElem, true);
+                cp_async16_or_zero(dst + kStep * S::kRowBytes, at + kv + i * kRowsPerCopy * D * kElem, true);
             }
             if constexpr (I8) {                           // lanes 0-15 the keys' scales, 16-31 the values'
                 const int64_t r = ((int64_t)page * a.pool.n_kv_heads + ahead_hk) * a.pool.page_size + slot + (lane & 15);
@@ -603,28 +613,28 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
         }
     };
 
-    // ---- q: warp w takes heads w, w + 4, ..., a lane D / 32 components, from global memory to registers
+    // ---- q: a warp takes every 4th (8th) head, a lane D / 32 components, from global memory to registers
     // (load_q), to 16 bits in shared memory (store_q), from there as the products' 8-column operand:
     // pair (2j, 2j + 1) and (2j + 8, 2j + 9) of each 16 components; an int8 row's words hold 4 components
     // in order, so there the pairs are (4j, 4j + 1) and (4j + 2, 4j + 3), in K and q alike
-    constexpr int kQWords = D / 64;
-    uint32_t q_in[S::kHeads / kWarps][kQWords];
+    constexpr int kQWords = D / 64, kQWarps = kWarps * S::kPair;
+    uint32_t q_in[S::kHeads / kQWarps][kQWords];
     uint32_t qf[S::kQInRegs ? NT : 1][S::kQInRegs ? kMt : 1][2];
     auto load_q = [&](const Place &p) {
         const int first = p.unit % a.n_groups * S::kHeads;
         const __nv_bfloat16 *q = a.q + p.b * a.q_stride + (int64_t)(p.unit / a.n_groups * a.group + first) * D;
 #pragma unroll
-        for (int i = 0; i < S::kHeads / kWarps; i++)
+        for (int i = 0; i < S::kHeads / kQWarps; i++)
 #pragma unroll
             for (int w = 0; w < kQWords; w++)
-                q_in[i][w] = first + warp + kWarps * i < a.group
-                                 ? reinterpret_cast<const uint32_t *>(q + (warp + kWarps * i) * D)[lane * kQWords + w]
+                q_in[i][w] = first + any_warp + kQWarps * i < a.group
+                                 ? reinterpret_cast<const uint32_t *>(q + (any_warp + kQWarps * i) * D)[lane * kQWords + w]
                                  : 0u;
     };
     auto store_q = [&]() {
 #pragma unroll
-        for (int i = 0; i < S::kHeads / kWarps; i++) {
-            const int h = warp + kWarps * i;
+        for (int i = 0; i < S::kHeads / kQWarps; i++) {
+            const int h = any_warp + kQWarps * i;
             if constexpr (I8) {
                 float top = 0.0f;
 #pragma unroll
@@ -648,7 +658,7 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
         }
     };
     auto q_word = [&](int nt, int c, int i) -> uint32_t {
-        return *reinterpret_cast<const uint32_t *>(q_s + (nt * 8 + g) * S::kQRow + 16 * c + (I8 ? 4 * j + 2 * i : 2 * j + 8 * i));
+        return *reinterpret_cast<const uint32_t *>(q_s + (nt * 8 + g) * S::kQRow + half * S::kPart + 16 * c + (I8 ? 4 * j + 2 * i : 2 * j + 8 * i));
     };
     float q_back[NT][2];                                  // an int8 pool's factors of heads 2j, 2j + 1
     auto take_q = [&]() {
@@ -683,6 +693,7 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
     take_q();
 
     int stage = 0;
+    [[maybe_unused]] int turn = 0;
     for (;;) {
         const int run = min(at.live.tiles - at.t, left);  // tiles of this unit
         float o[NT][kMt][4], m[NT][2], ms[NT][2], l[NT][2];   // ms: m - kLift, or 0 while there is no maximum
@@ -705,7 +716,7 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
             const uint32_t ks = ring_u + stage * S::kStage, vs = ks + kStep * S::kRowBytes;
             const unsigned char *tail = ring + stage * S::kStage + S::kRows;
             const unsigned mask = *reinterpret_cast<const unsigned *>(tail + (I8 ? 128 : 0));
-            if (mask) {
+            if (S::kPair == 2 || mask) {                  // a pair's warps meet in every step
                 // ---- S^T: keys g, g + 8 by heads 2j, 2j + 1
                 float s[NT][2][4];
 #pragma unroll
@@ -741,6 +752,22 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
                             for (int nt = 0; nt < NT; nt++)
                                 mma_f16(s[nt][x], a0, a1, a2, a3, q_of(nt, c + x, 0), q_of(nt, c + x, 1));
                         }
+                    }
+                }
+                if constexpr (S::kPair == 2) {            // the other half's part of the scores
+                    float4 *mine = reinterpret_cast<float4 *>(swap) + ((turn * kWarps + warp) * 2 + half) * 32 * NT + lane;
+                    const float4 *other = reinterpret_cast<const float4 *>(swap) + ((turn * kWarps + warp) * 2 + 1 - half) * 32 * NT + lane;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+                        mine[nt * 32] = make_float4(s[nt][0][0] + s[nt][1][0], s[nt][0][1] + s[nt][1][1],
+                                                    s[nt][0][2] + s[nt][1][2], s[nt][0][3] + s[nt][1][3]);
+                    xdna::named_bar(1 + warp, 64);
+                    turn ^= 1;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {     // in one order for both, so that both get the same
+                        const float4 x = half ? other[nt * 32] : mine[nt * 32], y = half ? mine[nt * 32] : other[nt * 32];
+                        s[nt][0][0] = x.x; s[nt][0][1] = x.y; s[nt][0][2] = x.z; s[nt][0][3] = x.w;
+                        s[nt][1][0] = y.x; s[nt][1][1] = y.y; s[nt][1][2] = y.z; s[nt][1][3] = y.w;
                     }
                 }
                 // ---- running maximum and weights
@@ -857,7 +884,7 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
 #pragma unroll
                 for (int x = 4; x < 32; x *= 2) l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], x);
                 m[nt][i] -= kLift;
-                if (g == 0) {
+                if (g == 0 && half == 0) {
                     join_m[warp][nt * 8 + 2 * j + i] = m[nt][i];
                     join_l[warp][nt * 8 + 2 * j + i] = l[nt][i];
                 }
@@ -889,10 +916,10 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
             for (int w = 0; w < kWarps; w++)
                 den += join_l[w][h] * (join_m[w][h] == top ? 1.0f : exp2_approx(join_m[w][h] - top));
         };
-        auto join_warps = [&](auto columns) {             // that many components at a time
-            constexpr int kCols = decltype(columns)::value, kRow = kCols + 4;
+        auto join_warps = [&](auto columns) {             // that many components of each part at a time
+            constexpr int kCols = decltype(columns)::value, kRow = kCols + 4, kLine = S::kPair * kCols / 4;
 #pragma unroll
-            for (int d0 = 0; d0 < D; d0 += kCols) {
+            for (int d0 = 0; d0 < S::kPart; d0 += kCols) {
                 if (d0) __syncthreads();
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
@@ -901,16 +928,17 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const int comp = 16 * c + (I8 ? 2 * g + (i >> 1) : g + 8 * (i >> 1));
-                            join_o[(warp * S::kHeads + nt * 8 + 2 * j + (i & 1)) * kRow + comp] =
+                            join_o[(any_warp * S::kHeads + nt * 8 + 2 * j + (i & 1)) * kRow + comp] =
                                 o[nt][d0 / 16 + c][i] * fac[nt][i & 1];
                         }
                 __syncthreads();
-                for (int x = tid; x < heads * (kCols / 4); x += 128) {
-                    const int h = x / (kCols / 4), c = x % (kCols / 4) * 4;
+                for (int x = tid; x < heads * kLine; x += kThreads) {
+                    const int h = x / kLine, part = x % kLine / (kCols / 4), c = x % (kCols / 4) * 4;
+                    const int to = part * S::kPart + d0 + c;
                     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                     for (int w = 0; w < kWarps; w++) {
-                        const float4 y = *reinterpret_cast<const float4 *>(&join_o[(w * S::kHeads + h) * kRow + c]);
+                        const float4 y = *reinterpret_cast<const float4 *>(&join_o[((w * S::kPair + part) * S::kHeads + h) * kRow + c]);
                         sum.x += y.x; sum.y += y.y; sum.z += y.z; sum.w += y.w;
                     }
                     if (whole) {
@@ -919,10 +947,10 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
                         const float inv = den == 0.0f ? 0.0f : 1.0f / den;
                         const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * inv, sum.y * inv),
                                              hi = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
-                        *reinterpret_cast<uint2 *>(a.out + ((int64_t)done.b * a.n_q_heads + h0 + h) * D + d0 + c) =
+                        *reinterpret_cast<uint2 *>(a.out + ((int64_t)done.b * a.n_q_heads + h0 + h) * D + to) =
                             make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
                     } else {
-                        *reinterpret_cast<float4 *>(a.part_o + ((int64_t)slot * S::kHeads + h) * D + d0 + c) = sum;
+                        *reinterpret_cast<float4 *>(a.part_o + ((int64_t)slot * S::kHeads + h) * D + to) = sum;
                     }
                 }
             }
@@ -931,7 +959,7 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
             join_warps(std::integral_constant<int, S::kJoinCols>{});
         } else {                                          // the ring is free: all at once
             join_o = reinterpret_cast<float *>(smem);
-            join_warps(std::integral_constant<int, D>{});
+            join_warps(std::integral_constant<int, S::kPart>{});
         }
         if (tid < heads) {
             float top, den;
@@ -961,8 +989,8 @@ __global__ void __launch_bounds__(128, (AttnShape<D, I8, NT>::kCtas)) attention_
                     if (!last) break;
                     __threadfence();
                     const bool final = n <= kJoinWays;
-                    // 128 / heads threads a head: the weights once, then their columns
-                    const int per_head = 128 / heads, h = tid / per_head;
+                    // kThreads / heads threads a head: the weights once, then their columns
+                    const int per_head = kThreads / heads, h = tid / per_head;
                     if (h < heads) {
                         const int64_t hop = (int64_t)2 * stride * S::kHeads;    // from part to part, in rows
                         const int64_t row0 = (int64_t)slot_of(0) * S::kHeads + h, row1 = (int64_t)slot_of(1) * S::kHeads + h - hop;
@@ -1063,8 +1091,8 @@ cudaError_t launch_attention(AttnArgs a, int sms, cudaStream_t st) {
     if (a.window) keys = std::min<int64_t>(keys, a.window);
     const int64_t tiles = units * ((keys + kStep - 1 + kTileKeys - 1) / kTileKeys + S::kEndCost);
     const int grid = (int)std::min<int64_t>((int64_t)sms * S::kCtas, tiles);
-    if ((tiles + 8) * (grid + 8) < 0x7fffffff) attention_kernel<D, I8, NT, true><<<grid, 128, S::kSmem, st>>>(a);
-    else attention_kernel<D, I8, NT, false><<<grid, 128, S::kSmem, st>>>(a);
+    if ((tiles + 8) * (grid + 8) < 0x7fffffff) attention_kernel<D, I8, NT, true><<<grid, S::kThreads, S::kSmem, st>>>(a);
+    else attention_kernel<D, I8, NT, false><<<grid, S::kThreads, S::kSmem, st>>>(a);
     return cudaGetLastError();
 }
 template <int D>
