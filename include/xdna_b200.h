@@ -530,13 +530,14 @@ int xdna_subsample_conv2d(const uint16_t *x_dev, int B, int ci, int hin, int win
  * pages shared by many streams, attention of one new token over it, the residual RMS norm that
  * feeds xdna_gemm_i8, and the last step from logits to the next token.  Pointers are device
  * pointers on the current device (for a cache: its device), work is asynchronous on `stream`,
- * nothing is allocated or waited for in a call (all of them may be captured in a CUDA graph);
- * 0, or -1 with xdna_last_error() set and nothing enqueued.
+ * nothing is allocated or waited for in a call (all of them may be captured in a CUDA graph), and
+ * what a call reads may not change before it has run; 0, or -1 with xdna_last_error() set and
+ * nothing enqueued.
  *
  * A paged cache describes caller-owned K and V pools of n_layers layers: element c of the row of
  * (layer, page, head, slot) lies at layer * stride_layer + page * stride_page + head *
- * stride_head + slot * stride_slot + c, in elements, K and V alike (two strides of 0: the
- * contiguous [layer][page][head][slot][c]).  kv_type 0: bf16; 1: int8 with one f32 scale per row,
+ * stride_head + slot * stride_slot + c, in elements, K and V alike (stride_page, stride_head and
+ * stride_slot all 0: the contiguous [layer][page][head][slot][c]).  kv_type 0: bf16; 1: int8 with one f32 scale per row,
  * k_scale / v_scale [n_layers][n_pages][n_kv_heads][page_size] (value = whole number * scale).
  * head_dim 64, 128 or 256; rows 16-byte aligned.  A block table (int32, [n_seqs][table_width],
  * rows table_stride apart) names the page of each page_size positions of a stream; entries past
@@ -562,8 +563,8 @@ void xdna_paged_cache_free(XdnaPagedCache *c);
  * multiple of 16 up to head_dim, the other components pass.  q_out [n_tokens][n_q_heads][head_dim]
  * bf16, disjoint from the inputs.  bf16 pools: rounded once; int8 pools, per row: scale =
  * max|x| / 127 (1 for a zero row), whole number = x * (127 * (1 / max|x|)), each step rounded to
- * f32, then half to even.  No two tokens
- * of a call may be the same position of one stream. */
+ * f32, then half to even (a NaN makes the scale NaN).  No two tokens of a call may be the same
+ * position of one stream. */
 int xdna_paged_append(XdnaPagedCache *c, int layer, int n_tokens, int n_q_heads, int src_f32, const void *q,
                       int64_t q_stride, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
                       const int32_t *tok_seq, const int32_t *tok_pos, const int32_t *block_table, int n_seqs,
@@ -573,8 +574,9 @@ int xdna_paged_append(XdnaPagedCache *c, int layer, int n_tokens, int n_q_heads,
  * q k^T) v over the stream's positions max(0, seq_lens - window) .. seq_lens - 1 (window 0: all);
  * q bf16, streams q_stride elements apart; query head h reads K/V head h / (n_q_heads /
  * n_kv_heads).  Scores, softmax and sums in f32, the weights to 16 bits of mantissa.  A stream
- * of no positions (seq_lens <= 0), or whose every score is -inf, gives zeros.  lse (NULL: none) [n_seqs][n_q_heads] f32: the
- * log of the sum of exponentials, -inf for no positions.  out may not overlap q. */
+ * of no positions (seq_lens <= 0), or whose every score is -inf, gives zeros.  lse (NULL: none)
+ * [n_seqs][n_q_heads] f32: the log of the sum of exponentials, -inf for no positions.  out may not
+ * overlap q. */
 int xdna_paged_attention(XdnaPagedCache *c, int layer, const uint16_t *q, int64_t q_stride, int n_q_heads,
                          const int32_t *block_table, int n_seqs, int table_width, int64_t table_stride,
                          const int32_t *seq_lens, float scale, int window, uint16_t *out, float *lse, void *stream);

@@ -652,6 +652,9 @@ def test_refusals(X, dev):
                       (dict(q=z(4, 4, 64), block_table=z(4, 2, t=I32), seq_lens=z(4, t=I32)), "max_seqs")):
         with pytest.raises(X.XdnaError, match=what):
             c.attend(**{**dict(q=q, block_table=table, seq_lens=lens), **bad})
+    one = q.data_ptr()
+    assert X.lib().xdna_paged_attention(c.handle, 0, one, 256, 4, one, 3, 1 << 26, 1 << 26, one, 0.125, 0, one, None, None) == -1
+    assert "2^29" in X.last_error()
     k, pos = z(3, 2, 64), z(3, t=I32)
     good = dict(q=q, k=k, v=k, tok_seq=None, tok_pos=pos, block_table=table)
     for bad in (dict(k=k.float()), dict(k=z(3, 3, 64)), dict(q=z(2, 4, 64)), dict(tok_pos=pos.long()),

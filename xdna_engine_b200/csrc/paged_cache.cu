@@ -1281,7 +1281,9 @@ int xdna_paged_attention(XdnaPagedCache *c, int layer, const uint16_t *q, int64_
     if (n_q_heads < 1 || n_q_heads > 65535 || n_q_heads % g.n_kv_heads)
         return fail(me + "n_q_heads not a multiple of the cache's K/V heads");
     if (n_q_heads / g.n_kv_heads > kMaxUnitHeads * kMaxGroups) return fail(me + "more than 128 query heads per K/V head");
-    if ((int64_t)table_width * g.page_size > 0x40000000) return fail(me + "more than 2^30 positions in a table row");
+    // 128 streams' tiles are summed in 32 bits, and so is a CTA's share
+    if ((int64_t)table_width * g.page_size > 0x20000000) return fail(me + "more than 2^29 positions in a table row");
+    if ((double)n_seqs * n_q_heads * table_width * g.page_size > 1e13) return fail(me + "more than 10^13 positions of all heads");
     if (window < 0 || !(scale > 0.0f)) return fail(me + "negative window or scale not above 0");
     if (q_stride < (int64_t)n_q_heads * g.head_dim || q_stride % 8 || !aligned16(q) || !aligned16(out))
         return fail(me + "q_stride below the heads' width, or rows not 16-byte aligned");
