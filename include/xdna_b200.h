@@ -538,7 +538,7 @@ int xdna_subsample_conv2d(const uint16_t *x_dev, int B, int ci, int hin, int win
  * (layer, page, head, slot) lies at layer * stride_layer + page * stride_page + head *
  * stride_head + slot * stride_slot + c, in elements, K and V alike (stride_page, stride_head and
  * stride_slot all 0: the contiguous [layer][page][head][slot][c]).  kv_type 0: bf16; 1: int8 with one f32 scale per row,
- * k_scale / v_scale [n_layers][n_pages][n_kv_heads][page_size] (value = whole number * scale).
+ * k_scale / v_scale [n_layers][n_pages][n_kv_heads][page_size] (value = whole number * scale, scales not negative).
  * head_dim 64, 128 or 256; rows 16-byte aligned.  A block table (int32, [n_seqs][table_width],
  * rows table_stride apart) names the page of each page_size positions of a stream; entries past
  * a stream's length are never read.  The handle holds a workspace and a status word: calls on

@@ -117,7 +117,7 @@ def rope_table(n_positions, rot_dim, theta=10000.0, device="cuda"):
 class PagedCache:
     """A paged key-value cache over the caller's pools k and v: tensors [n_pages, n_kv_heads,
     page_size, head_dim] (or with a leading [n_layers]), bf16, or int8 with k_scale and v_scale
-    f32 of the same shape without head_dim, contiguous.  k and v may be strided views of one kind (the
+    f32 of the same shape without head_dim, contiguous, not negative.  k and v may be strided views of one kind (the
     last dimension contiguous).  The pools are kept alive by this object.  Calls on one object run in
     one stream at a time."""
 
