@@ -1,0 +1,64 @@
+"""Edges of the serving ops: what a call meets at the ends of its ranges, against definitions in 64 bits.
+
+Tolerances are derived where they are used."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+BF16, F32, F64, I8, I32 = torch.bfloat16, torch.float32, torch.float64, torch.int8, torch.int32
+
+
+@pytest.fixture(scope="module")
+def X():
+    import xdna_engine_b200 as X
+    from xdna_engine_b200 import _build
+    _build.build()
+    return X
+
+
+@pytest.fixture(scope="module")
+def dev(X):
+    d = X.Device(0)
+    yield d
+    d.close()
+
+
+def rng(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def i32(x):
+    return torch.tensor(x, dtype=I32, device="cuda")
+
+
+# ------------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("d,hq,hkv", [(64, 32, 8), (128, 32, 8), (256, 8, 8), (128, 32, 2)])
+def test_attention_weights_are_f32(X, dev, d, hq, hkv):
+    """bf16 pools: the weights keep the 24 bits of f32.
+
+    Two keys, of values 0 and v, and scores below 1 with one product each that is not 0: o = v p / (1 + p).  In
+    units of 2^-24 p is off by 8 (scale log2 e, its constant, the product and the difference, for both scores) and 4
+    (the hardware exponential), the sum, 1 / sum and the last product by 1 each and the accumulated terms by 6: 21, below
+    2^-19.  So the output is the bf16 nearest to something within 2^-19 of o.  Weights of 16 bits are off by
+    up to 2^-18 and miss that in some of these 2 million places."""
+    g = rng(d + hkv)
+    n = 2**21 // (hq * d)
+    k, v = (torch.zeros(n, hkv, 16, d, dtype=BF16, device="cuda") for _ in "kv")
+    k[:, :, :2, 0] = torch.rand(n, hkv, 2, generator=g, device="cuda").mul(2).sub(1).to(BF16)
+    v[:, :, 1] = torch.randn(n, hkv, d, generator=g, device="cuda").to(BF16)
+    q = torch.randn(n, hq, d, generator=g, device="cuda").to(BF16)
+    q[..., 0] = 0.5 + 0.5 * torch.rand(n, hq, generator=g, device="cuda").to(BF16)
+    c = X.PagedCache(dev, k, v, max_seqs=n)
+    out = c.attend(q, torch.arange(n, dtype=I32, device="cuda")[:, None], torch.full((n,), 2, dtype=I32, device="cuda"),
+                   scale=1.0)
+    c.check()
+    s = k[:, :, :2, 0].to(F64).repeat_interleave(hq // hkv, 1) * q[..., :1].to(F64)
+    o = torch.softmax(s, -1)[..., 1:] * v[:, :, 1].to(F64).repeat_interleave(hq // hkv, 1)
+    ends = [(o * (1 + e)).float().to(BF16) for e in (-2.0**-19, 2.0**-19)]       # f32 first: 2^-24 more
+    lo, hi = torch.minimum(*ends), torch.maximum(*ends)
+    assert int(((out < lo) | (out > hi)).sum()) == 0

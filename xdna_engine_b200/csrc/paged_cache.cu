@@ -252,8 +252,9 @@ __global__ void __launch_bounds__(256, 6) append_kernel(const AppendArgs a) {
 // runs on over the share's units without a break, its own running maximum and sum, no barrier
 // until a unit's end, where the warps' parts are added.  S^T = K q^T and o^T += V^T p^T are m16n8k16
 // products with the keys (the components) in the 16-row operand, so that 8 query heads fill the 8
-// columns and fewer heads waste nothing but columns.  The weights p are used as two 16-bit terms,
-// which keeps the output's error that of its own rounding.  Keys past the end, before the window or on
+// columns and fewer heads waste nothing but columns.  The weights p are used as three bf16 terms, which
+// hold all of an f32 (of two terms, 17 bits, the output comes to the other bf16 neighbour four times as often as
+// of an f32 sum; one stream of 4k takes 0.4 us less with them, larger calls the same), or two fp16 ones.  Keys past the end, before the window or on
 // a bad page are zero-filled in shared memory and masked: what lies in the pool there is not read.
 //
 // bf16 pools: bf16 products.  int8 pools: fp16 products, to which a whole number converts in 5/4
@@ -361,20 +362,23 @@ __device__ __forceinline__ uint32_t f16x2_of_u8(uint32_t word, uint32_t sel) {
     const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&u), *reinterpret_cast<const __half2 *>(&off));
     return *reinterpret_cast<const uint32_t *>(&d);
 }
-// (x, y) as the 16-bit pair nearest and the pair of what that leaves
-template <bool F16>
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t &hi, uint32_t &lo) {
-    if constexpr (F16) {
-        const __half2 h = __floats2half2_rn(x, y);
-        const float2 f = __half22float2(h);
-        const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
-        hi = *reinterpret_cast<const uint32_t *>(&h);
-        lo = *reinterpret_cast<const uint32_t *>(&r);
-    } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-        hi = *reinterpret_cast<const uint32_t *>(&h);
-        const __nv_bfloat162 r = __floats2bfloat162_rn(x - xdna::bf16lo(hi), y - xdna::bf16hi(hi));
-        lo = *reinterpret_cast<const uint32_t *>(&r);
+// (x, y) as 16-bit pairs, each the nearest to what the ones before it leave
+template <bool F16, int N>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        if constexpr (F16) {
+            const __half2 h = __floats2half2_rn(x, y);
+            const float2 f = __half22float2(h);
+            t[n] = *reinterpret_cast<const uint32_t *>(&h);
+            x -= f.x;
+            y -= f.y;
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+            t[n] = *reinterpret_cast<const uint32_t *>(&h);
+            x -= xdna::bf16lo(t[n]);
+            y -= xdna::bf16hi(t[n]);
+        }
     }
 }
 
@@ -398,6 +402,7 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
     constexpr int kChunks = S::kRowBytes / 16, kRowsPerCopy = kChunks >= 32 ? 1 : 32 / kChunks, kCopies = kStep / kRowsPerCopy;
     constexpr int kMt = S::kPart / 16, kElem = I8 ? 1 : 2, kThreads = S::kThreads;
     constexpr float kLift = I8 ? 14.0f : 0.0f;            // weights reach up to 2^kLift
+    constexpr int kTerms = I8 ? 2 : 3;                    // 16-bit terms of a weight
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float join_m[kWarps][S::kHeads], join_l[kWarps][S::kHeads];
     __shared__ int last;
@@ -813,7 +818,7 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
                         }
                     }
                 }
-                uint32_t ph[NT][2], pl[NT][2];
+                uint32_t pt[NT][2][kTerms];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     float p[4];
@@ -822,12 +827,12 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
                         p[i] = exp2_approx(s[nt][0][i] - ms[nt][i & 1]);
                         l[nt][i & 1] += I8 ? exp2_approx(den[nt][i] - ms[nt][i & 1]) : p[i];
                     }
-                    split_pair<I8>(p[0], p[1], ph[nt][0], pl[nt][0]);
-                    split_pair<I8>(p[2], p[3], ph[nt][1], pl[nt][1]);
+                    split_pair<I8>(p[0], p[1], pt[nt][0]);
+                    split_pair<I8>(p[2], p[3], pt[nt][1]);
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        ph[nt][i] = transpose8x8(ph[nt][i]);
-                        pl[nt][i] = transpose8x8(pl[nt][i]);
+                    for (int x = 0; x < kTerms; x++) {
+                        pt[nt][0][x] = transpose8x8(pt[nt][0][x]);
+                        pt[nt][1][x] = transpose8x8(pt[nt][1][x]);
                     }
                 }
                 // ---- o^T += V^T p^T; an int8 word's bytes are components (2g, 2g + 1) of two keys: the
@@ -840,8 +845,9 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
                         ldsm4_trans(v, vs + rv * S::kRowBytes + (((2 * c + ((lane >> 3) & 1)) ^ swv) * 16));
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
-                            mma_bf16(o[nt][c], v[0], v[1], v[2], v[3], ph[nt][0], ph[nt][1]);
-                            mma_bf16(o[nt][c], v[0], v[1], v[2], v[3], pl[nt][0], pl[nt][1]);
+#pragma unroll
+                            for (int x = 0; x < kTerms; x++)
+                                mma_bf16(o[nt][c], v[0], v[1], v[2], v[3], pt[nt][0][x], pt[nt][1][x]);
                         }
                     }
                 } else {
@@ -857,8 +863,9 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
                             const uint32_t a2 = f16x2_of_u8(v[2 * x + 1], 0x4240), a3 = f16x2_of_u8(v[2 * x + 1], 0x4341);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
-                                mma_f16(o[nt][c + x], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-                                mma_f16(o[nt][c + x], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+#pragma unroll
+                                for (int y = 0; y < kTerms; y++)
+                                    mma_f16(o[nt][c + x], a0, a1, a2, a3, pt[nt][0][y], pt[nt][1][y]);
                             }
                         }
                     }
