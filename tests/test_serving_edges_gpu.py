@@ -62,3 +62,58 @@ def test_attention_weights_are_f32(X, dev, d, hq, hkv):
     ends = [(o * (1 + e)).float().to(BF16) for e in (-2.0**-19, 2.0**-19)]       # f32 first: 2^-24 more
     lo, hi = torch.minimum(*ends), torch.maximum(*ends)
     assert int(((out < lo) | (out > hi)).sum()) == 0
+
+
+# --------------------------------------------------------------------------------- streams
+def busy(stream, ms=20):
+    """Keep `stream` at work for some milliseconds."""
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(int(ms * 1.9e6))
+
+
+@pytest.mark.parametrize("b,v", [(3, 100003), (2, 262144)])
+def test_a_given_streams_workspace_is_its_own(X, b, v):
+    """process_logits on a stream that is still at work: what the current stream allocates and writes
+    meanwhile is neither the call's workspace nor its outputs."""
+    g = rng(v)
+    side = torch.cuda.Stream()
+    x = torch.randn(b, v, generator=g, device="cuda")
+    torch.cuda.synchronize()
+    for size in (X.lib().xdna_logits_workspace(b, v), b * v * 4, b * 8):
+        busy(side)
+        out, ids = X.process_logits(x, stream=side.cuda_stream)
+        mine = [torch.full((size,), 0xff, dtype=torch.uint8, device="cuda") for _ in range(4)]
+        torch.cuda.synchronize()
+        assert all(bool((m == 0xff).all()) for m in mine)
+        assert torch.equal(out, x) and torch.equal(ids, x.argmax(1))
+
+
+def test_a_given_streams_outputs_are_its_own(X, dev):
+    """Outputs that a call on a given stream allocates are not memory that the current stream's earlier work
+    still writes; the default stream (0) may be named too."""
+    g = rng(21)
+    side = torch.cuda.Stream()
+    m, d = 64, 1024
+    x, w = torch.randn(m, d, generator=g, device="cuda").to(BF16), torch.ones(d, device="cuda")
+    res = torch.randn(m, d, generator=g, device="cuda")
+    pool = torch.randn(m, 2, 16, 64, generator=g, device="cuda").to(BF16)
+    c = X.PagedCache(dev, pool, pool.clone())
+    q, k = (torch.randn(m, h, 64, generator=g, device="cuda").to(BF16) for h in (8, 2))
+    at, table = torch.full((m,), 15, dtype=I32, device="cuda"), torch.arange(m, dtype=I32, device="cuda")[:, None]
+    lg = torch.randn(m, 2000, generator=g, device="cuda")
+    calls = [lambda **s: X.rmsnorm_residual_i8(x, w, residual=res, **s),
+             lambda **s: c.append(q, k, k, None, at, table, **s),
+             lambda **s: c.attend(q, table, at, **s),
+             lambda **s: X.process_logits(lg, **s)]
+    flat = lambda t: [t] if torch.is_tensor(t) else [y for y in t if y is not None]  # noqa: E731
+    for call in calls:
+        want = flat(call())
+        torch.cuda.synchronize()
+        busy(torch.cuda.current_stream())
+        for t in want:                                    # freed at once, written late
+            torch.empty_like(t).fill_(7)
+        late = flat(call(stream=side.cuda_stream))
+        again = flat(call(stream=0))
+        torch.cuda.synchronize()
+        for a, b, e in zip(late, again, want):
+            assert torch.equal(a, e) and torch.equal(b, e)

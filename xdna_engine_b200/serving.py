@@ -6,6 +6,10 @@ the C ABI on the tensors' memory.  All of them are asynchronous on `stream` (a r
 None: torch's current stream of the tensors' device, so that torch's own ordering holds), and
 leave every tensor where it is: a tensor of the wrong type, shape, layout or device is refused with
 ValueError before anything is enqueued, and what the C ABI refuses raises XdnaError.
+
+With a `stream` given, what a call allocates (a workspace, outputs that were not passed in) is memory of
+that stream, which torch gives out again only behind that stream's work.  To order the inputs before the
+call and the outputs after it, and to keep the inputs until the stream has read them, is then the caller's.
 """
 from __future__ import annotations
 
@@ -103,7 +107,19 @@ def _rows(x, m, d, dev, name):
 # the raw stream and the current device without building objects (2 us of a small call), where torch has that
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _new(shape, dtype, device, stream, strides=None):
+    """An uninitialised tensor for a call on `stream` (None: the current one; 0 and 1: the default one)."""
+    if stream is not None:
+        of = torch.cuda.ExternalStream(stream, device=device) if stream > 1 else torch.cuda.default_stream(device)
+        with torch.cuda.stream(of):
+            return _new(shape, dtype, device, None, strides)
+    if strides is not None:
+        return torch.empty_strided(shape, strides, dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
 
 
 def rope_table(n_positions, rot_dim, theta=10000.0, device="cuda"):
@@ -165,7 +181,7 @@ class PagedCache:
         if q is not None:
             hq, qs = _heads(q, src, n, d, dev, "q")
             if q_out is None:
-                q_out = torch.empty(n, hq, d, dtype=torch.bfloat16, device=self.device)
+                q_out = _new((n, hq, d), torch.bfloat16, self.device, stream)
         if rope is not None:
             rows, rot = rope.shape
         n_seqs, width, ts = _table(block_table, dev)
@@ -191,7 +207,7 @@ class PagedCache:
         if n_seqs != n:
             raise ValueError(f"block_table: want {n} rows, got {n_seqs}")
         if out is None:
-            out = torch.empty(n, hq, d, dtype=torch.bfloat16, device=self.device)
+            out = _new((n, hq, d), torch.bfloat16, self.device, stream)
         if n == 0:
             return out
         if (_L or _lib()).xdna_paged_attention(
@@ -240,7 +256,7 @@ def rmsnorm_residual_i8(x, gamma, residual=None, eps=1e-6, unit_offset=False, q8
         rs = _rows(residual, m, d, dev, "residual")
         res_f32 = residual.dtype is torch.float32
         if residual_out is None:
-            residual_out = torch.empty_strided((m, d), (rs, 1), dtype=residual.dtype, device=x.device)
+            residual_out = _new((m, d), residual.dtype, x.device, stream, (rs, 1))
         elif residual_out is not residual and (
                 residual_out.dtype is not residual.dtype or _rows(residual_out, m, d, dev, "residual_out") != rs):
             raise ValueError("residual_out: want the type and row stride of residual")
@@ -248,9 +264,9 @@ def rmsnorm_residual_i8(x, gamma, residual=None, eps=1e-6, unit_offset=False, q8
         raise ValueError("residual_out without a residual")
     if quantize:
         if q8 is None:
-            q8 = torch.empty(m, d, dtype=torch.int8, device=x.device)
+            q8 = _new((m, d), torch.int8, x.device, stream)
         if scale is None:
-            scale = torch.empty(m, dtype=torch.float32, device=x.device)
+            scale = _new((m,), torch.float32, x.device, stream)
     elif q8 is not None or scale is not None:
         raise ValueError("q8 or scale with quantize=False")
     if m == 0:
@@ -284,17 +300,17 @@ def process_logits(logits, history=None, history_start=None, n_prompt=None, repe
     i32, f32 = torch.int32, torch.float32
     ls = _rows(logits, b, v, dev, "logits")
     if out is None:
-        out = torch.empty(b, v, dtype=f32, device=logits.device)
+        out = _new((b, v), f32, logits.device, stream)
     os_ = _rows(out, b, v, dev, "out")
     if out.dtype is not f32:
         raise ValueError(f"out: want f32, got {out.dtype}")
     if ids is None:
-        ids = torch.empty(b, dtype=torch.int64, device=logits.device)
+        ids = _new((b,), torch.int64, logits.device, stream)
     if b == 0:
         return out, ids
     L = _L or _lib()
     # rows of several clusters of CTAs need room for their chunks' choices
-    work = torch.empty(L.xdna_logits_workspace(b, v), dtype=torch.uint8, device=logits.device) if v > 60000 else None
+    work = _new((L.xdna_logits_workspace(b, v),), torch.uint8, logits.device, stream) if v > 60000 else None
     n = 0 if history is None else history.numel()
     e = 0 if bias is None else bias.numel()
     words = (v + 31) // 32
