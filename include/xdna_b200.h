@@ -590,8 +590,8 @@ int xdna_paged_cache_check(XdnaPagedCache *c, void *stream);
  * (x_f32 / res_f32) f32, rows x_stride / res_stride elements apart; gamma f32 [D].  Outputs, each
  * nullable but not all: residual_out [M][D] (type of residual; rows res_stride apart; may be
  * residual itself), y_bf16 [M][D], and q8 [M][D] with scale [M] (both or none): scale = max|y| /
- * 127 (1 for a zero row), q8 = r g * (127 * (1 / max|r g|)) half to even, the A operand of xdna_gemm_i8
- * with rows_per_clip 1.  1 <= D <= 16384. */
+ * 127 (1 for a zero row), q8 = r g * (127 * (1 / max|r g|)) half to even (a NaN makes the scale NaN), the A
+ * operand of xdna_gemm_i8 with rows_per_clip 1.  1 <= D <= 16384. */
 int xdna_rmsnorm_residual_i8(const void *x, int x_f32, int64_t x_stride, const void *residual, int res_f32,
                              int64_t res_stride, const float *gamma, int unit_offset, float eps, int M, int D,
                              void *residual_out, uint16_t *y_bf16, int8_t *q8, float *scale, void *stream);

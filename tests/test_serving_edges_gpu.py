@@ -117,3 +117,34 @@ def test_a_given_streams_outputs_are_its_own(X, dev):
         torch.cuda.synchronize()
         for a, b, e in zip(late, again, want):
             assert torch.equal(a, e) and torch.equal(b, e)
+
+
+# ------------------------------------------------------------------------------------- norm
+@pytest.mark.parametrize("x_type,res_type", [(BF16, BF16), (F32, None), (BF16, F32)])
+@pytest.mark.parametrize("d", [40, 1152, 4096, 5120, 16384, 37, 865, 2434, 10001])
+def test_norm_keeps_what_is_not_finite(X, d, x_type, res_type):
+    """Rows with one NaN, of nothing but NaN, of zeros and one NaN, with an infinity, and a NaN in gamma: not a
+    finite row in any output; the rows beside them are what they are alone."""
+    g = rng(d)
+    m = 9
+    x = torch.randn(m, d, generator=g, device="cuda").to(x_type)
+    res = None if res_type is None else torch.randn(m, d, generator=g, device="cuda").to(res_type)
+    w = torch.randn(d, generator=g, device="cuda")
+    good = [0, 2, 4, 6, 8]
+    alone = [t[good] for t in (X.rmsnorm_residual_i8(x, w, residual=res)[:2])]
+    x[1, d // 3] = math.nan
+    x[3] = math.nan
+    x[5] = 0
+    x[7, d - 1] = -math.inf
+    if res is not None:
+        res[5] = 0
+    x[5, d // 2] = math.nan
+    y = torch.empty(m, d, dtype=BF16, device="cuda")
+    q8, scale, _ = X.rmsnorm_residual_i8(x, w, residual=res, y=y)
+    values = q8 * scale[:, None]
+    assert torch.isnan(scale[[1, 3, 5, 7]]).all() and torch.isnan(values[[1, 3, 5, 7]]).all()
+    assert torch.isnan(y[[1, 3, 5]].float()).all() and torch.isnan(y[7, d - 1].float())
+    assert torch.equal(q8[good], alone[0]) and torch.equal(scale[good], alone[1])
+    w[d - 2] = math.nan
+    q8, scale, _ = X.rmsnorm_residual_i8(x[good], w, residual=None if res is None else res[good])
+    assert torch.isnan(scale).all()

@@ -146,7 +146,8 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_kernel(const NormArgs a) {
     }
     int phase = 0;
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x, phase ^= 1) {
-        float r[P][N], sum = 0.0f, top = 0.0f;
+        float r[P][N], sum = 0.0f;
+        unsigned bits = 0;                                // magnitudes ordered as bits: a NaN is the largest and makes the scale NaN
 #pragma unroll
         for (int p = 0; p < P; p++) {
             if (place(p) >= a.D) break;
@@ -169,31 +170,32 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_kernel(const NormArgs a) {
             for (int k = 0; k < N; k++) {
                 sum = fmaf(r[p][k], r[p][k], sum);
                 r[p][k] = __fmul_rn(r[p][k], kAhead ? g[p][k] : w[k]);
-                top = fmaxf(top, fabsf(r[p][k]));
+                bits = max(bits, __float_as_uint(fabsf(r[p][k])));
             }
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));   // not negative: ordered as bits
-        if (lane == 0) red[phase][warp] = make_float2(sum, top);
+        bits = __reduce_max_sync(0xffffffffu, bits);
+        if (lane == 0) red[phase][warp] = make_float2(sum, __uint_as_float(bits));
         __syncthreads();
         if constexpr (kThreads <= 256) {
             sum = red[phase][0].x;
             for (int w = 1; w < warps; w++) {
                 sum += red[phase][w].x;
-                top = fmaxf(top, red[phase][w].y);
+                bits = max(bits, __float_as_uint(red[phase][w].y));
             }
-            top = fmaxf(top, red[phase][0].y);
+            bits = max(bits, __float_as_uint(red[phase][0].y));
         } else {
             const float2 part = lane < warps ? red[phase][lane] : make_float2(0.0f, 0.0f);
             sum = part.x;
 #pragma unroll
             for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(part.y)));
+            bits = __reduce_max_sync(0xffffffffu, __float_as_uint(part.y));
         }
+        const float top = __uint_as_float(bits);
         const float inv = rsqrtf(__fdiv_rn(sum, (float)a.D) + a.eps);
         // below 127 / FLT_MAX the factor would be infinite: such a row counts as zero
-        const bool zero = !(top > 3.8e-37f);
+        const bool zero = top <= 3.8e-37f;
         const float to8 = zero ? 0.0f : __fmul_rn(__frcp_rn(top), 127.0f);
 #pragma unroll
         for (int p = 0; p < P; p++) {
