@@ -64,6 +64,38 @@ def test_attention_weights_are_f32(X, dev, d, hq, hkv):
     assert int(((out < lo) | (out > hi)).sum()) == 0
 
 
+@pytest.mark.parametrize("d,slots,kv", [(256, 2**23, "bf16"), (128, 2**24, "bf16"), (256, 2**24, "int8"), (256, 2**23 + 48, "bf16")])
+def test_attention_past_32_bits_within_a_page(X, dev, d, slots, kv):
+    """Rows whose bytes lie past 2^31 in their page: a contiguous cache of one page.  A page of zeros whose last
+    301 rows count; without a window every row does, at weight 1."""
+    g = rng(d + slots % 97)
+    n, window = slots - 5, 301
+    pool = torch.zeros(1, 1, slots, d, dtype=BF16 if kv == "bf16" else I8, device="cuda")
+    scales = [None, None] if kv == "bf16" else [torch.full((1, 1, slots), 2.0**-5 * (i + 1), device="cuda") for i in range(2)]
+    rows = torch.randn(window, d, generator=g, device="cuda") if kv == "bf16" else \
+        torch.randint(-127, 128, (window, d), generator=g, device="cuda")
+    pool[0, 0, n - window:n] = rows.to(pool.dtype)
+    c = X.PagedCache(dev, pool, pool, *scales)
+    q = torch.randn(1, 4, d, generator=g, device="cuda").to(BF16)
+    table, lens = i32([[0]]), i32([n])
+    live = pool[0, 0, n - window:n].to(F64)
+    k, v = (live, live) if kv == "bf16" else (live / 32, live / 16)
+    s = q[0].to(F64) @ k.T * d ** -0.5
+    o = torch.softmax(s, 1) @ v
+    # the scores' f32 sums, 2^-23 of sum|q k| each, and their weights' share; bf16 outputs
+    ds = float((q[0].to(F64).abs() @ k.abs().T).max()) * d ** -0.5 * (d + 4) * 2.0**-23
+    rel = 2 * ds + 2.0**-16 + window * 2.0**-23
+    out = c.attend(q, table, lens, window=window)
+    c.check()
+    bound = o.abs() * 1.01 * 2.0**-8 + rel * (torch.softmax(s, 1) @ v.abs())
+    assert float(((out[0].to(F64) - o).abs() - bound).max()) <= 0
+    lse = torch.empty(1, 4, device="cuda")
+    c.attend(q.zero_(), table, lens, lse=lse)
+    c.check()
+    # a sum of n ones: every part of it is a whole number below 2^24, exact
+    assert float((lse.to(F64) - math.log(n)).abs().max()) <= 2.0**-19 + math.log(n) * 2.0**-22
+
+
 # --------------------------------------------------------------------------------- streams
 def busy(stream, ms=20):
     """Keep `stream` at work for some milliseconds."""

@@ -576,7 +576,7 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
         if (a.dense_steps && pos >= ahead.live.x && pos + kStep <= ahead.live.y && (unsigned)page < (unsigned)a.pool.n_pages) {
             // 16 whole rows side by side
             const int slot = a.page_shift >= 0 ? pos & ((1 << a.page_shift) - 1) : pos % a.pool.page_size;
-            const unsigned char *at = kb + page * a.pool.sp * kElem + (slot + lane_row) * (D * kElem) + lane_chunk * 16;
+            const unsigned char *at = kb + page * a.pool.sp * kElem + (int64_t)(slot + lane_row) * (D * kElem) + lane_chunk * 16;
 #pragma unroll
             for (int i = 0; i < kCopies; i++) {
                 const uint32_t dst = base + swizzled(i * kRowsPerCopy + lane_row, lane_chunk);
