@@ -180,3 +180,32 @@ def test_norm_keeps_what_is_not_finite(X, d, x_type, res_type):
     w[d - 2] = math.nan
     q8, scale, _ = X.rmsnorm_residual_i8(x[good], w, residual=None if res is None else res[good])
     assert torch.isnan(scale).all()
+
+
+# ----------------------------------------------------------------------------------- logits
+@pytest.mark.parametrize("v", [70, 5000, 100003])
+def test_logits_offsets_are_held_within_the_lists(X, v):
+    """Starts that fall, lie below 0 or past the lists, down to -2^31 and up to 2^31 - 1: as if they were held to [0,
+    length], with no entries where a row's end lies before its start."""
+    big = 2**31 - 1
+    g = rng(v)
+    starts = [5, -big - 1, 3, big, -3, 2, 9, 9, 8, -big - 1, big]
+    b = len(starts) - 1
+    x = torch.randn(b, v, generator=g, device="cuda")
+    ids = torch.randperm(70, generator=g, device="cuda")[:8].int()
+    add = torch.randn(8, generator=g, device="cuda")
+    want = x.clone()
+    for r in range(b):
+        lo, hi = max(0, starts[r]), min(8, starts[r + 1])
+        for j in range(lo, hi):
+            want[r, int(ids[j])] += add[j]
+    out, best = X.process_logits(x, bias_ids=ids, bias=add, bias_start=i32(starts))
+    assert torch.equal(out, want) and torch.equal(best, want.argmax(1))
+    minus = torch.linspace(0.5, 2, b, device="cuda")
+    want = x.clone()
+    for r in range(b):
+        lo, hi = max(0, starts[r]), min(8, starts[r + 1])
+        for j in range(lo, hi):
+            want[r, int(ids[j])] -= minus[r]
+    out, best = X.process_logits(x, history=ids, history_start=i32(starts), presence=minus)
+    assert torch.equal(out, want) and torch.equal(best, want.argmax(1))

@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 2) logits_kernel(const LogitsA
         h1 = min(a.n_hist, h1);
         gen = min(max(0, gen), 0x7fffffff - h0) + h0;
         e0 = max(0, e0);
-        e1 = min(a.n_bias, e1);
+        e1 = max(e0, min(a.n_bias, e1));                  // so that e1 - e0 does not wrap
         int biased = e1 - e0 > tid ? a.bias_ids[e0 + tid] : -1;
         int ids[kAhead];
         auto ahead = [&](int j0) {
