@@ -573,7 +573,7 @@ int xdna_paged_append(XdnaPagedCache *c, int layer, int n_tokens, int n_q_heads,
 /* Attention of one new token per stream: out [n_seqs][n_q_heads][head_dim] bf16 = softmax(scale
  * q k^T) v over the stream's positions max(0, seq_lens - window) .. seq_lens - 1 (window 0: all);
  * q bf16, streams q_stride elements apart; query head h reads K/V head h / (n_q_heads /
- * n_kv_heads).  Scores, softmax and sums in f32; int8 pools: the weights to 22 bits of mantissa.  A stream
+ * n_kv_heads).  Scores, softmax and sums in f32.  A stream
  * of no positions (seq_lens <= 0), or whose every score is -inf, gives zeros.  lse (NULL: none)
  * [n_seqs][n_q_heads] f32: the log of the sum of exponentials, -inf for no positions.  out may not
  * overlap q. */

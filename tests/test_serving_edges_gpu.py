@@ -6,6 +6,8 @@ import math
 import pytest
 
 torch = pytest.importorskip("torch")
+from test_serving_gpu import attention_64, check_attention, make_pool  # noqa: E402
+
 pytestmark = pytest.mark.gpu
 
 BF16, F32, F64, I8, I32 = torch.bfloat16, torch.float32, torch.float64, torch.int8, torch.int32
@@ -94,6 +96,66 @@ def test_attention_past_32_bits_within_a_page(X, dev, d, slots, kv):
     c.check()
     # a sum of n ones: every part of it is a whole number below 2^24, exact
     assert float((lse.to(F64) - math.log(n)).abs().max()) <= 2.0**-19 + math.log(n) * 2.0**-22
+
+
+@pytest.mark.parametrize("d,hkv,n", [(64, 1, 40000), (128, 2, 70000), (256, 1, 33000)])
+def test_int8_values_of_scale_zero(X, dev, d, hkv, n):
+    """Value rows of scale 0 give zeros and leave the log-sum-exp alone."""
+    g = rng(n)
+    p = make_pool(g, "int8", [n, 50], hkv, 16, d)
+    p["k_scale"] = p["k_scale"].nan_to_num(0.0)
+    p["v_scale"] = torch.zeros_like(p["v_scale"])
+    q = torch.randn(2, 4 * hkv, d, generator=g, device="cuda").mul(0.1).to(BF16)
+    c = X.PagedCache(dev, p["k"], p["v"], p["k_scale"], p["v_scale"])
+    lse = torch.empty(2, 4 * hkv, device="cuda")
+    out = c.attend(q, p["table"], i32([n, 50]), lse=lse)
+    c.check()
+    check_attention(out, lse, attention_64(q, p, [n, 50], d ** -0.5, 0))
+    assert not out.any()
+
+
+@pytest.mark.parametrize("v_scale", [1e-30, 1e-12, 1.0, 1e6])
+@pytest.mark.parametrize("d,hq,hkv", [(64, 4, 1), (128, 32, 2), (256, 16, 2)])
+def test_int8_values_of_any_scale(X, dev, d, hq, hkv, v_scale):
+    """The same bounds hold whatever the values' scales are, and as scores climb through a stream."""
+    g = rng(d)
+    lens = [700, 3, 1500]
+    p = make_pool(g, "int8", lens, hkv, 16, d)
+    p["v_scale"] *= v_scale
+    climb = torch.linspace(1, 8, p["k"].shape[1], device="cuda")
+    p["k_scale"] *= climb[None, :, None, None]
+    q = torch.randn(3, hq, d, generator=g, device="cuda").to(BF16)
+    c = X.PagedCache(dev, p["k"], p["v"], p["k_scale"], p["v_scale"])
+    lse = torch.empty(3, hq, device="cuda")
+    out = c.attend(q, p["table"], i32(lens), lse=lse)
+    c.check()
+    check_attention(out, lse, attention_64(q, p, lens, d ** -0.5, 0))
+
+
+@pytest.mark.parametrize("at", [0, 100, 299])
+@pytest.mark.parametrize("gap", [0, 12, 20, 40, 80])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_int8_zero_value_row_that_dominates(X, dev, d, gap, at):
+    """A key whose value row is zero, of scale 1 as append leaves it, `gap` above the others' scores: their values
+    still come out to bf16's rounding."""
+    g = rng(d + gap + at)
+    p = make_pool(g, "int8", [300], 1, 16, d)
+    p["k"][..., 1:] = 0
+    p["k"][..., 0].clamp_(-64, 64)
+    p["k_scale"] = torch.full_like(p["k_scale"], 1 / 64)
+    p["v_scale"] = torch.where(p["v_scale"].isnan(), 1.0, p["v_scale"])
+    page, slot = int(p["table"][0, at // 16]), at % 16
+    p["k"][0, page, 0, slot, 0] = 127
+    p["k_scale"][0, page, 0, slot] = (1 + gap) / 127
+    p["v"][0, page, 0, slot] = 0
+    p["v_scale"][0, page, 0, slot] = 1.0
+    q = torch.zeros(1, 4, d, dtype=BF16, device="cuda")
+    q[..., 0] = 1.0
+    c = X.PagedCache(dev, p["k"], p["v"], p["k_scale"], p["v_scale"])
+    lse = torch.empty(1, 4, device="cuda")
+    out = c.attend(q, p["table"], i32([300]), scale=1.0, lse=lse)
+    c.check()
+    check_attention(out, lse, attention_64(q, p, [300], 1.0, 0))
 
 
 # --------------------------------------------------------------------------------- streams

@@ -254,14 +254,14 @@ __global__ void __launch_bounds__(256, 6) append_kernel(const AppendArgs a) {
 // products with the keys (the components) in the 16-row operand, so that 8 query heads fill the 8
 // columns and fewer heads waste nothing but columns.  The weights p are used as three bf16 terms, which
 // hold all of an f32 (of two terms, 17 bits, the output comes to the other bf16 neighbour four times as often as
-// of an f32 sum; one stream of 4k takes 0.4 us less with them, larger calls the same), or two fp16 ones.  Keys past the end, before the window or on
-// a bad page are zero-filled in shared memory and masked: what lies in the pool there is not read.
+// of an f32 sum; one stream of 4k takes 0.4 us less with them, larger calls the same).  Keys past the end,
+// before the window or on a bad page are zero-filled in shared memory and masked: what lies in the pool there is not read.
 //
-// bf16 pools: bf16 products.  int8 pools: fp16 products, to which a whole number converts in 5/4
-// instructions (bf16: 2), at 4 KB a step of D = 128 the difference between the instruction rate and
-// HBM as the bound.  q is scaled there by a power of two per head to fp16's upper range; a
-// value's scale v_scale goes into the exponent, w_j = exp2(s_j + log2 v_scale_j - max + 14), which fp16
-// holds whatever the scales.
+// int8 pools: a value's scale goes into its key's weight, p v_scale in f32.  V's whole numbers become bf16, the only
+// 16-bit type that holds such weights whatever they are: as fp16 (4 x 64k 99 us, now 116) those 2^39 below the
+// largest vanish, be its value row zero or not.  K's become fp16, in 5/4 instructions a pair to bf16's 17/4, and q is
+// scaled for that by a power of two per head to fp16's upper range: components of q down to 2^-20 of the
+// head's largest are exact, the others off by 2^-39 of it at most.
 //
 // Measured: 64 streams of 0 to 8k, 32/8 heads x 128, pages of 16, 183 us (5.9 TB/s, 90 % of a copy); 4 x 64k
 // in int8 101 us (5.5 TB/s; issue-bound next); 32 streams of 0 to 2k, 12 heads x 64, 27.5 us; one stream
@@ -350,11 +350,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float log2_approx(float x) {
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // bytes sel of a word of int8 + 128 (the word with its sign bits flipped) as an fp16 pair, exactly:
 // 0x6400 | u is 1024 + u
 __device__ __forceinline__ uint32_t f16x2_of_u8(uint32_t word, uint32_t sel) {
@@ -362,23 +357,25 @@ __device__ __forceinline__ uint32_t f16x2_of_u8(uint32_t word, uint32_t sel) {
     const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&u), *reinterpret_cast<const __half2 *>(&off));
     return *reinterpret_cast<const uint32_t *>(&d);
 }
-// (x, y) as 16-bit pairs, each the nearest to what the ones before it leave
-template <bool F16, int N>
+// the low bytes of a word's halves, signed, as a bf16 pair, exactly.  With u = x + 128, 0x4300 | u is 128 + u up to
+// 255 and 2 u from 256, of which x = f / 2 - 128 - max(128 - f / 2, 0)
+__device__ __forceinline__ uint32_t bf16x2_of_s8(uint32_t word) {
+    const uint32_t f = (word & 0x00ff00ffu) ^ 0x43804380u;
+    uint32_t r, y;
+    asm("{.reg .b32 half, back;\n\tmov.b32 half, 0x3f003f00;\n\tmov.b32 back, 0xbf00bf00;\n\t"
+        "fma.rn.relu.bf16x2 %0, %2, back, %3;\n\tfma.rn.bf16x2 %1, %2, half, %4;\n\t}" : "=&r"(r), "=r"(y) : "r"(f), "r"(0x43004300u), "r"(0xc300c300u));
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&y), *reinterpret_cast<const __nv_bfloat162 *>(&r));
+    return *reinterpret_cast<const uint32_t *>(&d);
+}
+// (x, y) as bf16 pairs, each the nearest to what the ones before it leave
+template <int N>
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[N]) {
 #pragma unroll
     for (int n = 0; n < N; n++) {
-        if constexpr (F16) {
-            const __half2 h = __floats2half2_rn(x, y);
-            const float2 f = __half22float2(h);
-            t[n] = *reinterpret_cast<const uint32_t *>(&h);
-            x -= f.x;
-            y -= f.y;
-        } else {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-            t[n] = *reinterpret_cast<const uint32_t *>(&h);
-            x -= xdna::bf16lo(t[n]);
-            y -= xdna::bf16hi(t[n]);
-        }
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        t[n] = *reinterpret_cast<const uint32_t *>(&h);
+        x -= xdna::bf16lo(t[n]);
+        y -= xdna::bf16hi(t[n]);
     }
 }
 
@@ -401,8 +398,7 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
     using S = AttnShape<D, I8, NT>;
     constexpr int kChunks = S::kRowBytes / 16, kRowsPerCopy = kChunks >= 32 ? 1 : 32 / kChunks, kCopies = kStep / kRowsPerCopy;
     constexpr int kMt = S::kPart / 16, kElem = I8 ? 1 : 2, kThreads = S::kThreads;
-    constexpr float kLift = I8 ? 14.0f : 0.0f;            // weights reach up to 2^kLift
-    constexpr int kTerms = I8 ? 2 : 3;                    // 16-bit terms of a weight
+    constexpr int kTerms = 3;                             // bf16 terms of a weight
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float join_m[kWarps][S::kHeads], join_l[kWarps][S::kHeads];
     __shared__ int last;
@@ -701,7 +697,7 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
     [[maybe_unused]] int turn = 0;
     for (;;) {
         const int run = min(at.live.tiles - at.t, left);  // tiles of this unit
-        float o[NT][kMt][4], m[NT][2], ms[NT][2], l[NT][2];   // ms: m - kLift, or 0 while there is no maximum
+        float o[NT][kMt][4], m[NT][2], ms[NT][2], l[NT][2];   // ms: m, or 0 while there is no maximum
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -781,10 +777,8 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
                 if constexpr (I8) {
                     const float *sc = reinterpret_cast<const float *>(tail);
                     f0 = sc[g]; f1 = sc[g + 8];
-                    v0 = log2_approx(sc[16 + g] < 1e-30f ? 1e-30f : sc[16 + g]);   // a NaN stays one
-                    v1 = log2_approx(sc[24 + g] < 1e-30f ? 1e-30f : sc[24 + g]);
+                    v0 = sc[16 + g]; v1 = sc[24 + g];
                 }
-                float den[NT][4];                         // the exponents of the sum's terms, s[.][0] the weights'
                 bool up = false;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
@@ -793,9 +787,8 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
                         float x = (s[nt][0][i] + s[nt][1][i]) * (i < 2 ? f0 : f1);
                         if constexpr (I8) x *= q_back[nt][i & 1];
                         x = (i < 2 ? ok0 : ok1) ? x : -INFINITY;
-                        den[nt][i] = x;
-                        s[nt][0][i] = I8 ? x + (i < 2 ? v0 : v1) : x;
-                        up |= s[nt][0][i] > m[nt][i & 1];
+                        s[nt][0][i] = x;
+                        up |= x > m[nt][i & 1];
                     }
                 if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -808,7 +801,7 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
                             for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                             corr[i] = top == m[nt][i] ? 1.0f : exp2_approx(m[nt][i] - top);
                             m[nt][i] = top;
-                            ms[nt][i] = top == -INFINITY ? 0.0f : top - kLift;
+                            ms[nt][i] = top == -INFINITY ? 0.0f : top;
                             l[nt][i] *= corr[i];
                         }
 #pragma unroll
@@ -825,10 +818,11 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         p[i] = exp2_approx(s[nt][0][i] - ms[nt][i & 1]);
-                        l[nt][i & 1] += I8 ? exp2_approx(den[nt][i] - ms[nt][i & 1]) : p[i];
+                        l[nt][i & 1] += p[i];
+                        if constexpr (I8) p[i] *= i < 2 ? v0 : v1;
                     }
-                    split_pair<I8>(p[0], p[1], pt[nt][0]);
-                    split_pair<I8>(p[2], p[3], pt[nt][1]);
+                    split_pair(p[0], p[1], pt[nt][0]);
+                    split_pair(p[2], p[3], pt[nt][1]);
 #pragma unroll
                     for (int x = 0; x < kTerms; x++) {
                         pt[nt][0][x] = transpose8x8(pt[nt][0][x]);
@@ -856,16 +850,14 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
                         uint32_t v[4];
                         ldsm4_trans(v, vs + r * S::kRowBytes + (((c + (lane >> 4)) ^ sw) * 16));
 #pragma unroll
-                        for (int x = 0; x < 4; x++) v[x] ^= 0x80808080u;
-#pragma unroll
                         for (int x = 0; x < 2; x++) {
-                            const uint32_t a0 = f16x2_of_u8(v[2 * x], 0x4240), a1 = f16x2_of_u8(v[2 * x], 0x4341);
-                            const uint32_t a2 = f16x2_of_u8(v[2 * x + 1], 0x4240), a3 = f16x2_of_u8(v[2 * x + 1], 0x4341);
+                            const uint32_t a0 = bf16x2_of_s8(v[2 * x]), a1 = bf16x2_of_s8(v[2 * x] >> 8);
+                            const uint32_t a2 = bf16x2_of_s8(v[2 * x + 1]), a3 = bf16x2_of_s8(v[2 * x + 1] >> 8);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                                 for (int y = 0; y < kTerms; y++)
-                                    mma_f16(o[nt][c + x], a0, a1, a2, a3, pt[nt][0][y], pt[nt][1][y]);
+                                    mma_bf16(o[nt][c + x], a0, a1, a2, a3, pt[nt][0][y], pt[nt][1][y]);
                             }
                         }
                     }
@@ -890,7 +882,6 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
             for (int i = 0; i < 2; i++) {
 #pragma unroll
                 for (int x = 4; x < 32; x *= 2) l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], x);
-                m[nt][i] -= kLift;
                 if (g == 0 && half == 0) {
                     join_m[warp][nt * 8 + 2 * j + i] = m[nt][i];
                     join_l[warp][nt * 8 + 2 * j + i] = l[nt][i];
