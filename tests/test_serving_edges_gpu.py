@@ -271,3 +271,29 @@ def test_logits_offsets_are_held_within_the_lists(X, v):
             want[r, int(ids[j])] -= minus[r]
     out, best = X.process_logits(x, history=ids, history_start=i32(starts), presence=minus)
     assert torch.equal(out, want) and torch.equal(best, want.argmax(1))
+
+
+# --------------------------------------------------------------------------------- refusals
+def test_shapes_of_the_same_size_are_refused(X, dev):
+    """A tensor of the right size whose dimensions lie in another order."""
+    z = lambda *s, t=BF16: torch.zeros(*s, dtype=t, device="cuda")  # noqa: E731
+    pool, scale = z(4, 2, 16, 64, t=I8), z(4, 2, 16, t=F32)
+    nhd = z(4, 16, 2, 64, t=I8).transpose(1, 2)
+    for kw in (dict(k=nhd, v=nhd, k_scale=z(4, 16, 2, t=F32), v_scale=z(4, 16, 2, t=F32)),
+               dict(k=pool, v=pool, k_scale=scale, v_scale=z(4, 16, 2, t=F32)),
+               dict(k=pool, v=pool, k_scale=scale[None], v_scale=scale[None])):
+        with pytest.raises(ValueError, match="_scale"):
+            X.PagedCache(dev, **kw)
+    c = X.PagedCache(dev, nhd, nhd, scale, scale)
+    q, table, lens = z(3, 4, 64), z(3, 2, t=I32), z(3, t=I32)
+    for bad in (dict(out=z(4, 3, 64)), dict(lse=z(4, 3, t=F32))):
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            c.attend(q, table, lens, **bad)
+    with pytest.raises(ValueError, match="q_out"):
+        c.append(q, z(3, 2, 64), z(3, 2, 64), None, lens, table, q_out=z(4, 3, 64))
+    x, w = z(3, 64), z(64, t=F32)
+    for bad in (dict(q8=z(64, 3, t=I8)), dict(y=z(64, 3))):
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            X.rmsnorm_residual_i8(x, w, **bad)
+    with pytest.raises(ValueError, match="mask"):
+        X.process_logits(z(3, 100, t=F32), mask=z(4, 3, t=I32))

@@ -260,8 +260,8 @@ __global__ void __launch_bounds__(256, 6) append_kernel(const AppendArgs a) {
 // int8 pools: a value's scale goes into its key's weight, p v_scale in f32.  V's whole numbers become bf16, the only
 // 16-bit type that holds such weights whatever they are: as fp16 (4 x 64k 99 us, now 116) those 2^39 below the
 // largest vanish, be its value row zero or not.  K's become fp16, in 5/4 instructions a pair to bf16's 17/4, and q is
-// scaled for that by a power of two per head to fp16's upper range: components of q down to 2^-20 of the
-// head's largest are exact, the others off by 2^-39 of it at most.
+// scaled for that by a power of two per head to fp16's upper range: components of q down to 2^-30 of the
+// head's largest are exact, the others off by 2^-38 of it at most.
 //
 // Measured: 64 streams of 0 to 8k, 32/8 heads x 128, pages of 16, 183 us (5.9 TB/s, 90 % of a copy); 4 x 64k
 // in int8 101 us (5.5 TB/s; issue-bound next); 32 streams of 0 to 2k, 12 heads x 64, 27.5 us; one stream

@@ -65,8 +65,18 @@ def _lib():
 
 # These run in front of every launch, and a small launch is bound by them: plain attribute reads, and no
 # message is formatted unless it is raised.
+def _dense(t, dtype, shape, dev, name):
+    """The address of a contiguous tensor of this type and shape on device dev (None: NULL)."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name}: want a contiguous {dtype} tensor {tuple(shape)} on GPU {dev}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}, strides {t.stride()}")
+    return t.data_ptr()
+
+
 def _flat(t, dtype, n, dev, name):
-    """The address of a contiguous tensor of n elements of this type on device dev (None: NULL)."""
+    """The address of a contiguous tensor of n elements, a list of any shape, of this type on device dev (None: NULL)."""
     if t is None:
         return None
     if t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
@@ -151,11 +161,10 @@ class PagedCache:
         if i8 != (k_scale is not None) or i8 != (v_scale is not None):
             raise ValueError("int8 pools, and only they, have scales")
         five = k if k.dim() == 5 else k[None]
-        rows = k.numel() // k.shape[-1]
         c = _PagedConfig(int(i8), five.shape[0], five.shape[1], five.shape[3], five.shape[2], five.shape[4], max_seqs,
                          k.data_ptr(), v.data_ptr(), *five.stride()[:4],
-                         _flat(k_scale, torch.float32, rows, dev, "k_scale"),
-                         _flat(v_scale, torch.float32, rows, dev, "v_scale"))
+                         _dense(k_scale, torch.float32, k.shape[:-1], dev, "k_scale"),
+                         _dense(v_scale, torch.float32, k.shape[:-1], dev, "v_scale"))
         self.handle = None
         h = _lib().xdna_paged_cache_create(device.handle, C.byref(c))
         if not h:
@@ -191,8 +200,8 @@ class PagedCache:
                 self.handle, layer, n, hq, src is torch.float32, None if q is None else q.data_ptr(), qs, k.data_ptr(),
                 ks, v.data_ptr(), vs, _flat(tok_seq, torch.int32, n, dev, "tok_seq"),
                 _flat(tok_pos, torch.int32, n, dev, "tok_pos"), block_table.data_ptr(), n_seqs, width, ts,
-                _flat(rope, torch.float32, rows * rot, dev, "rope"), rows, rot, interleaved,
-                None if q is None else _flat(q_out, torch.bfloat16, n * hq * d, dev, "q_out"),
+                _dense(rope, torch.float32, (rows, rot), dev, "rope"), rows, rot, interleaved,
+                None if q is None else _dense(q_out, torch.bfloat16, (n, hq, d), dev, "q_out"),
                 _raw_stream(dev) if stream is None else stream):
             raise XdnaError(last_error())
         return q_out
@@ -213,7 +222,7 @@ class PagedCache:
         if (_L or _lib()).xdna_paged_attention(
                 self.handle, layer, q.data_ptr(), qs, hq, block_table.data_ptr(), n, width, ts,
                 _flat(seq_lens, torch.int32, n, dev, "seq_lens"), d ** -0.5 if scale is None else scale, window,
-                _flat(out, torch.bfloat16, n * hq * d, dev, "out"), _flat(lse, torch.float32, n * hq, dev, "lse"),
+                _dense(out, torch.bfloat16, (n, hq, d), dev, "out"), _dense(lse, torch.float32, (n, hq), dev, "lse"),
                 _raw_stream(dev) if stream is None else stream):
             raise XdnaError(last_error())
         return out
@@ -274,8 +283,8 @@ def rmsnorm_residual_i8(x, gamma, residual=None, eps=1e-6, unit_offset=False, q8
     if (_L or _lib()).xdna_rmsnorm_residual_i8(
             x.data_ptr(), x.dtype is torch.float32, xs, None if residual is None else residual.data_ptr(), res_f32, rs,
             _flat(gamma, torch.float32, d, dev, "gamma"), unit_offset, eps, m, d,
-            None if residual_out is None else residual_out.data_ptr(), _flat(y, torch.bfloat16, m * d, dev, "y"),
-            _flat(q8, torch.int8, m * d, dev, "q8"), _flat(scale, torch.float32, m, dev, "scale"),
+            None if residual_out is None else residual_out.data_ptr(), _dense(y, torch.bfloat16, (m, d), dev, "y"),
+            _dense(q8, torch.int8, (m, d), dev, "q8"), _flat(scale, torch.float32, m, dev, "scale"),
             _raw_stream(dev) if stream is None else stream):
         raise XdnaError(last_error())
     return q8, scale, residual_out
@@ -320,7 +329,7 @@ def process_logits(logits, history=None, history_start=None, n_prompt=None, repe
             _flat(repetition, f32, b, dev, "repetition"), _flat(frequency, f32, b, dev, "frequency"),
             _flat(presence, f32, b, dev, "presence"), _flat(bias_ids, i32, e, dev, "bias_ids"),
             _flat(bias, f32, e, dev, "bias"), e, _flat(bias_start, i32, b + 1, dev, "bias_start"),
-            _flat(mask, i32, b * words, dev, "mask"), words, out.data_ptr(), os_, _flat(ids, torch.int64, b, dev, "ids"),
+            _dense(mask, i32, (b, words), dev, "mask"), words, out.data_ptr(), os_, _flat(ids, torch.int64, b, dev, "ids"),
             None if work is None else work.data_ptr(), _raw_stream(dev) if stream is None else stream):
         raise XdnaError(last_error())
     return out, ids
