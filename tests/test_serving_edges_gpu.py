@@ -273,6 +273,22 @@ def test_logits_offsets_are_held_within_the_lists(X, v):
     assert torch.equal(out, want) and torch.equal(best, want.argmax(1))
 
 
+@pytest.mark.parametrize("v", [50, 100003])
+def test_logits_empty_lists(X, v):
+    """A step whose rows have no tokens yet, or no biases: lists of no entries are lists."""
+    g = rng(v)
+    x = torch.randn(3, v, generator=g, device="cuda")
+    none, start = torch.empty(0, dtype=I32, device="cuda"), i32([0] * 4)
+    one = torch.ones(3, device="cuda")
+    both = dict(history=none, history_start=start, n_prompt=i32([0, 0, 0]), repetition=one * 2, frequency=one, presence=one)
+    bias = dict(bias_ids=none, bias=none.float(), bias_start=start)
+    for kw in (both, bias, {**both, **bias}):
+        out, ids = X.process_logits(x, **kw)
+        assert torch.equal(out, x) and torch.equal(ids, x.argmax(1))
+    with pytest.raises(X.XdnaError, match="together"):
+        X.process_logits(x, history_start=start)
+
+
 # --------------------------------------------------------------------------------- refusals
 def test_shapes_of_the_same_size_are_refused(X, dev):
     """A tensor of the right size whose dimensions lie in another order."""

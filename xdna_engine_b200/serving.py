@@ -85,6 +85,12 @@ def _flat(t, dtype, n, dev, name):
     return t.data_ptr()
 
 
+def _list(t, start, dtype, n, dev, name):
+    """As _flat, for a list whose rows begin at `start`: torch's address of an empty tensor is 0, which is no list at
+    all, so that of `start`, where nothing is read, stands for it."""
+    return _flat(t, dtype, n, dev, name) or (None if t is None or start is None else start.data_ptr())
+
+
 def _heads(x, dtype, n, d, dev, name):
     """(heads, token stride) of an [n, heads, d] tensor with contiguous heads."""
     shape, s = x.shape, x.stride()
@@ -324,11 +330,11 @@ def process_logits(logits, history=None, history_start=None, n_prompt=None, repe
     e = 0 if bias is None else bias.numel()
     words = (v + 31) // 32
     if L.xdna_logits_process(
-            logits.data_ptr(), logits.dtype is f32, ls, b, v, _flat(history, i32, n, dev, "history"), n,
+            logits.data_ptr(), logits.dtype is f32, ls, b, v, _list(history, history_start, i32, n, dev, "history"), n,
             _flat(history_start, i32, b + 1, dev, "history_start"), _flat(n_prompt, i32, b, dev, "n_prompt"),
             _flat(repetition, f32, b, dev, "repetition"), _flat(frequency, f32, b, dev, "frequency"),
-            _flat(presence, f32, b, dev, "presence"), _flat(bias_ids, i32, e, dev, "bias_ids"),
-            _flat(bias, f32, e, dev, "bias"), e, _flat(bias_start, i32, b + 1, dev, "bias_start"),
+            _flat(presence, f32, b, dev, "presence"), _list(bias_ids, bias_start, i32, e, dev, "bias_ids"),
+            _list(bias, bias_start, f32, e, dev, "bias"), e, _flat(bias_start, i32, b + 1, dev, "bias_start"),
             _dense(mask, i32, (b, words), dev, "mask"), words, out.data_ptr(), os_, _flat(ids, torch.int64, b, dev, "ids"),
             None if work is None else work.data_ptr(), _raw_stream(dev) if stream is None else stream):
         raise XdnaError(last_error())
