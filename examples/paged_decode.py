@@ -13,8 +13,8 @@ One layer of the step, for any number of tokens of any streams:
     xdna_ffn_fused_bf16   the feed-forward's two products
 
 and at the end the LM head and process_logits: penalties, biases, grammar mask, the next token.  A
-prompt goes through the same step: its tokens are appended together, and token i attends over the
-first i + 1 positions as a stream of that length with the same pages.
+prompt goes through the same step: its tokens are appended together, max_tokens of them to a call, and token i
+attends over the first i + 1 positions as a stream of that length with the same pages.
 """
 import dataclasses
 import os
@@ -73,7 +73,7 @@ class PagedDecoder:
     """The model over a pool of pages; what stream owns which pages is the caller's business."""
 
     def __init__(self, device, cfg, weights, n_pages, page_size=16, kv="bf16", max_tokens=512):
-        self.cfg, self.w, self.dev = cfg, weights, f"cuda:{device.ordinal}"
+        self.cfg, self.w, self.dev, self.max_tokens = cfg, weights, f"cuda:{device.ordinal}", max_tokens
         shape = (cfg.n_layers, n_pages, cfg.n_kv_heads, page_size, cfg.head_dim)
         pools = [torch.zeros(shape, dtype=torch.bfloat16 if kv == "bf16" else torch.int8, device=self.dev) for _ in "kv"]
         scales = [None, None] if kv == "bf16" else [torch.ones(shape[:4], device=self.dev) for _ in "kv"]
@@ -155,9 +155,13 @@ class Server:
         s = self.streams[name] = dict(tokens=list(prompt), prompt=len(prompt), pages=[])
         n, dev = len(prompt), self.model.dev
         self._grow(s, n)
-        out = self.model.logits(torch.tensor(prompt, device=dev), torch.zeros(n, dtype=torch.int32, device=dev),
-                                torch.arange(n, dtype=torch.int32, device=dev), self._table([s]),
-                                rows=torch.tensor([n - 1], device=dev))
+        table = self._table([s])
+        for at in range(0, n, self.model.max_tokens):
+            piece = torch.tensor(prompt[at:at + self.model.max_tokens], device=dev)
+            k = piece.numel()
+            out = self.model.logits(piece, torch.zeros(k, dtype=torch.int32, device=dev),
+                                    torch.arange(at, at + k, dtype=torch.int32, device=dev), table,
+                                    rows=torch.tensor([k - 1], device=dev))
         self._next(out, [s])
 
     def step(self):
