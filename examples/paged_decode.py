@@ -152,8 +152,10 @@ class Server:
 
     def admit(self, name, prompt):
         """Run a prompt and choose the first token after it."""
-        s = self.streams[name] = dict(tokens=list(prompt), prompt=len(prompt), pages=[])
         n, dev = len(prompt), self.model.dev
+        if name in self.streams or n == 0 or -(-n // self.page_size) > min(self.width, len(self.free)):
+            raise ValueError(f"a stream {name!r} of {n} tokens: known already, empty, or too long for the free pages")
+        s = self.streams[name] = dict(tokens=list(prompt), prompt=n, pages=[])
         self._grow(s, n)
         table = self._table([s])
         for at in range(0, n, self.model.max_tokens):
@@ -167,6 +169,8 @@ class Server:
     def step(self):
         """One token for every stream, at its own position."""
         group, dev = list(self.streams.values()), self.model.dev
+        if not group:
+            return
         pos = [len(s["tokens"]) - 1 for s in group]
         for s, p in zip(group, pos):
             self._grow(s, p + 1)

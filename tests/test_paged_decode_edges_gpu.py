@@ -28,3 +28,22 @@ def test_prompts_longer_than_a_call(E, dev, n, max_tokens):  # noqa: F811
         seen = torch.tensor(sorted(set(prompt + new[:k])), device="cuda")
         x[seen] = torch.where(x[seen] > 0, x[seen] / 1.1, x[seen] * 1.1)
         assert float(x.max() - x[t]) <= 0.03 * 6 * float(x.std()), k
+
+
+def test_a_refused_prompt_leaves_the_server_as_it_was(E, dev):  # noqa: F811
+    """A prompt that the free pages or a table's width do not hold, and an empty one: no stream and no page is kept."""
+    cfg = E.Config(n_layers=1)
+    model = E.PagedDecoder(dev, cfg, E.make_weights(cfg, seed=1), 10)
+    server = E.Server(model, 10, width=8)
+    server.step()                                         # no streams yet: nothing to do
+    server.admit("a", [1, 2, 3])
+    for prompt in (list(range(300)), list(range(8 * 16 + 1)), []):
+        with pytest.raises(ValueError):
+            server.admit("b", prompt)
+        assert list(server.streams) == ["a"] and len(server.free) == 9
+    with pytest.raises(ValueError):
+        server.admit("a", [4])
+    server.admit("b", list(range(100)))
+    server.step()
+    model.check()
+    assert len(server.release("a")) == 2 and len(server.release("b")) == 2 and sorted(server.free) == list(range(10))
