@@ -158,6 +158,66 @@ def test_int8_zero_value_row_that_dominates(X, dev, d, gap, at):
     check_attention(out, lse, attention_64(q, p, [300], 1.0, 0))
 
 
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("d,hq,hkv", [(64, 8, 8), (128, 32, 8), (256, 8, 8), (64, 64, 4), (128, 64, 4), (256, 64, 4)])
+@pytest.mark.parametrize("b,window", [(64, 0), (150, 0), (150, 300000)])
+def test_attention_wide_tables(X, dev, d, hq, hkv, b, window, kv):
+    """A table of a million positions a stream, whose tiles need 64 bits to be shared out, gives the bits that a
+    narrow one gives: its CTAs and their shares are the same."""
+    g = rng(b + d)
+    lens = [(i * 37) % 1800 for i in range(b)]
+    p = make_pool(g, kv, lens, hkv, 16, d)
+    q = torch.randn(b, hq, d, generator=g, device="cuda").to(BF16)
+    c = X.PagedCache(dev, p["k"], p["v"], p["k_scale"], p["v_scale"], max_seqs=b)
+    wide = torch.full((b, 65536), -5, dtype=I32, device="cuda")
+    wide[:, : p["table"].shape[1]] = p["table"]
+    res = []
+    for table in (p["table"], wide):
+        lse = torch.empty(b, hq, device="cuda")
+        out = c.attend(q, table, i32(lens), lse=lse, window=window)
+        c.check()
+        res.append((out, lse))
+    assert torch.equal(res[0][0].view(torch.int16), res[1][0].view(torch.int16)) and torch.equal(res[0][1], res[1][1])
+    few = [0, 1, b // 2, b - 1, max(range(b), key=lambda i: lens[i])]
+    check_attention(out[few], lse[few], attention_64(q[few], dict(p, table=p["table"][few]), [lens[i] for i in few],
+                                                     d ** -0.5, 0))
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("page", [7, 24])
+@pytest.mark.parametrize("window", [0, 50])
+def test_attention_pages_that_cut_steps(X, dev, d, page, window, kv):
+    """Pages that are not whole steps of 16 keys, at the head sizes that lay their shared memory out otherwise."""
+    g = rng(d + page)
+    lens = [0, 5, 600, 99, 1025, 16, 1]
+    p = make_pool(g, kv, lens, 2, page, d)
+    for hq in (8, 32):
+        q = torch.randn(len(lens), hq, d, generator=g, device="cuda").to(BF16)
+        c = X.PagedCache(dev, p["k"], p["v"], p["k_scale"], p["v_scale"])
+        lse = torch.empty(len(lens), hq, device="cuda")
+        out = c.attend(q, p["table"], i32(lens), window=window, lse=lse)
+        c.check()
+        check_attention(out, lse, attention_64(q, p, lens, d ** -0.5, window))
+
+
+def test_attention_every_stream_as_alone(X, dev):
+    """A batch's streams each give what they give in a call of their own, to the joins' f32 rounding: the same parts
+    in other shares, 2^-19 of the sums, and one rounding to bf16 on either side."""
+    g = rng(77)
+    lens = [1] * 150 + [7000] + [33] * 100 + [300] * 49
+    p = make_pool(g, "bf16", lens, 8, 16, 128)
+    q = torch.randn(len(lens), 32, 128, generator=g, device="cuda").to(BF16)
+    c = X.PagedCache(dev, p["k"], p["v"], max_seqs=len(lens))
+    out = c.attend(q, p["table"], i32(lens)).float()
+    top = 0.0
+    for i, n in enumerate(lens):
+        one = c.attend(q[i:i + 1], p["table"][i:i + 1, :-(-n // 16)], i32([n]))[0].float()
+        top = max(top, float(((out[i] - one).abs() - one.abs() * 2.0**-7 - 2.0**-17).max()))
+    c.check()
+    assert top <= 0
+
+
 # --------------------------------------------------------------------------------- streams
 def busy(stream, ms=20):
     """Keep `stream` at work for some milliseconds."""
