@@ -373,3 +373,20 @@ def test_shapes_of_the_same_size_are_refused(X, dev):
             X.rmsnorm_residual_i8(x, w, **bad)
     with pytest.raises(ValueError, match="mask"):
         X.process_logits(z(3, 100, t=F32), mask=z(4, 3, t=I32))
+
+
+def test_pointers_off_their_elements(X, dev):
+    """The cache's C entries refuse 4-byte arrays that lie off 4 bytes, before anything is enqueued."""
+    z = lambda *s, t=BF16: torch.zeros(*s, dtype=t, device="cuda")  # noqa: E731
+    pool = z(4, 2, 16, 64)
+    c = X.PagedCache(dev, pool, pool.clone())
+    L, one = X.lib(), z(4096).data_ptr()
+    attend = dict(c=c.handle, layer=0, q=one, qs=256, hq=4, table=one, n=3, width=2, ts=2, lens=one, scale=0.125, window=0,
+                  out=one, lse=one, st=None)
+    for name in ("table", "lens", "lse"):
+        assert L.xdna_paged_attention(*{**attend, name: one + 2}.values()) == -1 and "aligned" in X.last_error(), name
+    append = dict(c=c.handle, layer=0, n=0, hq=4, f=0, q=one, qs=256, k=one, ks=128, v=one, vs=128, seq=one, pos=one, table=one,
+                  ns=3, width=2, ts=2, rope=None, rows=0, rot=0, inter=0, out=one, st=None)
+    assert L.xdna_paged_append(*append.values()) == 0
+    for name in ("seq", "pos", "table"):
+        assert L.xdna_paged_append(*{**append, name: one + 2}.values()) == -1 and "aligned" in X.last_error(), name

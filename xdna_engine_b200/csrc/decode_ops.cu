@@ -29,6 +29,11 @@ int fail(const std::string &m) {
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// the pointers that lie off their elements' boundary (NULL does not)
+template <typename... P>
+bool off_elements(size_t bytes, P... p) {
+    return ((reinterpret_cast<uintptr_t>(p) % bytes) | ...) != 0;
+}
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -610,6 +615,9 @@ int xdna_rmsnorm_residual_i8(const void *x, int x_f32, int64_t x_stride, const v
     if (M < 0 || D < 1 || D > 16384) return fail(me + "negative M, or D outside 1..16384");
     if (x_stride < D || ((residual || residual_out) && res_stride < D)) return fail(me + "a row stride below D");
     if (!(eps >= 0.0f)) return fail(me + "negative eps");
+    if (off_elements(x_f32 ? 4 : 2, x) || off_elements(res_f32 ? 4 : 2, residual, residual_out) ||
+        off_elements(4, gamma, scale) || off_elements(2, y_bf16))
+        return fail(me + "a pointer not aligned to its elements");
     if (M == 0) return 0;
     NormArgs a{x, residual, x_stride, res_stride, gamma, unit_offset, M, D, eps, residual_out,
                reinterpret_cast<__nv_bfloat16 *>(y_bf16), q8, scale};
@@ -652,6 +660,9 @@ int xdna_logits_process(const void *logits, int src_f32, int64_t logits_stride, 
     if (out == logits && (!src_f32 || (B > 1 && out_stride != logits_stride)))
         return fail(me + "out on bf16 logits, or on logits of another stride");
     if (B > 65535) return fail(me + "more than 65535 rows");
+    if (off_elements(src_f32 ? 4 : 2, logits) || off_elements(8, ids) ||
+        off_elements(4, out, history, history_start, n_prompt, repetition, frequency, presence, bias_ids, bias, bias_start, mask))
+        return fail(me + "a pointer not aligned to its elements");
     if (ids && xdna_logits_workspace(B, V) && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 8))
         return fail(me + "ids need a workspace, 8-byte aligned");
     if (B == 0) return 0;

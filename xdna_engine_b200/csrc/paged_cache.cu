@@ -44,6 +44,11 @@ int fail(const std::string &m) {
     return -1;
 }
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// the pointers that lie off their elements' boundary (NULL does not)
+template <typename... P>
+bool off_elements(size_t bytes, P... p) {
+    return ((reinterpret_cast<uintptr_t>(p) % bytes) | ...) != 0;
+}
 
 // a call on a cache leaves the caller's current device as it was
 struct OnDevice {
@@ -1159,6 +1164,7 @@ XdnaPagedCache *xdna_paged_cache_create(XdnaDevice *dev, const XdnaPagedCacheCon
     const int64_t st[4] = {g.stride_layer, g.stride_page, g.stride_head, g.stride_slot};
     const int ext[4] = {g.n_layers, g.n_pages, g.n_kv_heads, g.page_size};
     if (!aligned16(g.k) || !aligned16(g.v)) return refuse("pools not 16-byte aligned");
+    if (off_elements(4, g.k_scale, g.v_scale)) return refuse("scales not aligned to their elements");
     for (int i = 0; i < 4; i++)
         if (ext[i] > 1 && (st[i] < g.head_dim || st[i] % unit))
             return refuse("a stride below head_dim or not a multiple of 16 bytes");
@@ -1233,6 +1239,7 @@ int xdna_paged_append(XdnaPagedCache *c, int layer, int n_tokens, int n_q_heads,
     if (k_stride % unit || v_stride % unit || (q && q_stride % unit) || !aligned16(q) || !aligned16(k) ||
         !aligned16(v) || !aligned16(q_out) || !aligned16(rope))
         return fail(me + "rows not 16-byte aligned");
+    if (off_elements(4, tok_seq, tok_pos, block_table)) return fail(me + "a pointer not aligned to its elements");
     if (n_tokens == 0) return 0;
     OnDevice on(c->ordinal);
     if (!on.ok) return fail(me + "cannot select the cache's device");
@@ -1285,6 +1292,7 @@ int xdna_paged_attention(XdnaPagedCache *c, int layer, const uint16_t *q, int64_
     if (window < 0 || !(scale > 0.0f)) return fail(me + "negative window or scale not above 0");
     if (q_stride < (int64_t)n_q_heads * g.head_dim || q_stride % 8 || !aligned16(q) || !aligned16(out))
         return fail(me + "q_stride below the heads' width, or rows not 16-byte aligned");
+    if (off_elements(4, block_table, seq_lens, lse)) return fail(me + "a pointer not aligned to its elements");
     OnDevice on(c->ordinal);
     if (!on.ok) return fail(me + "cannot select the cache's device");
     AttnArgs a{};
