@@ -532,7 +532,7 @@ int xdna_subsample_conv2d(const uint16_t *x_dev, int B, int ci, int hin, int win
  * pointers on the current device (for a cache: its device), work is asynchronous on `stream`,
  * nothing is allocated or waited for in a call (all of them may be captured in a CUDA graph), and
  * what a call reads may not change before it has run; 0, or -1 with xdna_last_error() set and
- * nothing enqueued.
+ * nothing enqueued (also for a pointer off its elements' boundary).
  *
  * A paged cache describes caller-owned K and V pools of n_layers layers: element c of the row of
  * (layer, page, head, slot) lies at layer * stride_layer + page * stride_page + head *
@@ -542,7 +542,8 @@ int xdna_subsample_conv2d(const uint16_t *x_dev, int B, int ci, int hin, int win
  * head_dim 64, 128 or 256; rows 16-byte aligned.  A block table (int32, [n_seqs][table_width],
  * rows table_stride apart) names the page of each page_size positions of a stream; entries past
  * a stream's length are never read.  The handle holds a workspace and a status word: calls on
- * one handle run in one stream at a time.  max_seqs bounds the streams of one attention call. */
+ * one handle run in one stream at a time.  max_seqs (up to 65535) bounds the streams of one attention call.  At most
+ * 1024 K/V heads. */
 typedef struct {
     int kv_type, n_layers, n_pages, page_size, n_kv_heads, head_dim, max_seqs;
     void *k, *v;
@@ -562,8 +563,8 @@ void xdna_paged_cache_free(XdnaPagedCache *c);
  * turned by angle i: (a cos - b sin, b cos + a sin), each product and sum rounded to f32; rot_dim a
  * multiple of 16 up to head_dim, the other components pass.  q_out [n_tokens][n_q_heads][head_dim]
  * bf16, disjoint from the inputs.  bf16 pools: rounded once; int8 pools, per row: scale =
- * max|x| / 127 (1 for a zero row), whole number = x * (127 * (1 / max|x|)), each step rounded to
- * f32, then half to even (a NaN makes the scale NaN).  No two tokens of a call may be the same
+ * max|x| / 127 (1 for a zero row, as which one below 3.8e-37 counts), whole number = x * (127 * (1 / max|x|)), each
+ * step rounded to f32, then half to even (a NaN makes the scale NaN).  No two tokens of a call may be the same
  * position of one stream. */
 int xdna_paged_append(XdnaPagedCache *c, int layer, int n_tokens, int n_q_heads, int src_f32, const void *q,
                       int64_t q_stride, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
@@ -576,7 +577,8 @@ int xdna_paged_append(XdnaPagedCache *c, int layer, int n_tokens, int n_q_heads,
  * n_kv_heads).  Scores, softmax and sums in f32.  A stream
  * of no positions (seq_lens <= 0), or whose every score is -inf, gives zeros.  lse (NULL: none)
  * [n_seqs][n_q_heads] f32: the log of the sum of exponentials, -inf for no positions.  out may not
- * overlap q. */
+ * overlap q.  At most 128 query heads to a K/V head, 2^29 positions in a table row, 10^13 positions of all
+ * query heads. */
 int xdna_paged_attention(XdnaPagedCache *c, int layer, const uint16_t *q, int64_t q_stride, int n_q_heads,
                          const int32_t *block_table, int n_seqs, int table_width, int64_t table_stride,
                          const int32_t *seq_lens, float scale, int window, uint16_t *out, float *lse, void *stream);
@@ -590,8 +592,8 @@ int xdna_paged_cache_check(XdnaPagedCache *c, void *stream);
  * (x_f32 / res_f32) f32, rows x_stride / res_stride elements apart; gamma f32 [D].  Outputs, each
  * nullable but not all: residual_out [M][D] (type of residual; rows res_stride apart; may be
  * residual itself), y_bf16 [M][D], and q8 [M][D] with scale [M] (both or none): scale = max|y| /
- * 127 (1 for a zero row), q8 = r g * (127 * (1 / max|r g|)) half to even (a NaN makes the scale NaN), the A
- * operand of xdna_gemm_i8 with rows_per_clip 1.  1 <= D <= 16384. */
+ * 127 (1 for a zero row, as which one of max|r g| below 3.8e-37 counts), q8 = r g * (127 * (1 / max|r g|)) half to
+ * even (a NaN makes the scale NaN), the A operand of xdna_gemm_i8 with rows_per_clip 1.  1 <= D <= 16384. */
 int xdna_rmsnorm_residual_i8(const void *x, int x_f32, int64_t x_stride, const void *residual, int res_f32,
                              int64_t res_stride, const float *gamma, int unit_offset, float eps, int M, int D,
                              void *residual_out, uint16_t *y_bf16, int8_t *q8, float *scale, void *stream);

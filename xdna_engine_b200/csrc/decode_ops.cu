@@ -114,8 +114,8 @@ __device__ __forceinline__ void store_n(__nv_bfloat16 *p, const float (&v)[N]) {
 // scales both y and its maximum and drops out of the whole numbers.  kAhead: gamma stays in registers and
 // the next row's loads pass under the reduction and the outputs; without it (wide rows, whose
 // threads have no registers left) other CTAs of the SM do that.  N = 8 where every row is 16-byte
-// aligned, else N = 1.  Measured: 8192 x 4096 bf16 46.6 us, 5.0 TB/s (kAhead off: 50.6); 64 x 1152
-// 2.2 us; 4592 rows of 865, f32 and bf16 (N = 1) 16.5 us, 2.2 TB/s.
+// aligned, else N = 1.  Measured: 8192 x 4096 bf16 47.3 us, 5.0 TB/s (kAhead off: 50.6); 64 x 1152
+// 2.3 us; 4592 rows of 865, f32 and bf16 (N = 1) 16.5 us, 2.2 TB/s, bound by its 2- and 4-byte accesses.
 template <typename X, typename R, int N, int P, int kThreads, bool kAhead>
 __global__ void __launch_bounds__(kThreads) rmsnorm_kernel(const NormArgs a) {
     __shared__ float2 red[2][kThreads / 32];              // alternating, so that a row needs one barrier

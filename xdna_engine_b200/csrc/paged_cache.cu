@@ -132,8 +132,9 @@ __device__ __forceinline__ void store8(int8_t *p, const float (&x)[8], float inv
 // together, so that a lane holds both halves of its pairs; a row's D / 16 lanes lie side by side in
 // a warp, which gives the int8 row's maximum by shuffles.  4 or 2 bytes in and 2 or 1 out per element, so
 // HBM bounds it; a token's rotary row comes from L1 for all its heads but the first.  Measured: 8192 tokens
-// of 32/8 heads x 128, f32 in, 52.5 us (5.8 TB/s; several heads to a lane, with the rotary row kept in
-// registers: 60 us); 2003 tokens of 4/1 x 256 into int8 5.0 us; 64 tokens 2.5 us.
+// of 32/8 heads x 128, f32 in, 52.7 us (5.8 TB/s; several heads to a lane, with the rotary row kept in
+// registers: 60 us); 2003 tokens of 4/1 x 256 into int8 5.0 us; 64 tokens 2.7 us.  Six CTAs an SM leave 40
+// registers a thread and spill 20 to 32 bytes.
 template <int D, typename Src, bool I8>
 __global__ void __launch_bounds__(256, 6) append_kernel(const AppendArgs a) {
     constexpr int L = D / 16;
@@ -239,14 +240,14 @@ __global__ void __launch_bounds__(256, 6) append_kernel(const AppendArgs a) {
 //
 // For each stream b and K/V head, with the G query heads that share it:
 //   s_j = scale q.k_j,  m = max s_j,  l = sum exp(s_j - m),  o = sum exp(s_j - m) v_j / l
-// over the stream's live keys.  Every key and value is read once: 2 n D elements for 4 n G D
-// operations, at most G (bf16) or 2 G (int8) operations a byte, so HBM bounds it.
+// over the stream's live keys.  Up to 16 heads a group, every key and value is read once (of more, once for each 16):
+// 2 n D elements for 4 n G D operations, at most 16 (bf16) or 32 (int8) operations a byte, so HBM bounds it.
 //
 // Work split.  A unit is (stream, K/V head, group of up to 8 NT query heads); its keys are cut into
 // tiles of 16 keys per warp.  All units' tiles, laid end to end, are dealt to the CTAs in equal
 // contiguous shares, whatever the streams' lengths; a CTA walks its share unit by unit.  A unit's end
 // counts as kEndCost tiles, since its work there costs so much (32 ragged streams of 12 heads x 64, up
-// to 2k: 32.2 us at 0, 29.5 at 1, 27.4 at 2, 27.2 at 3).  A unit
+// to 2k: 32.2 us at 0, 29.5 at 1, 27.4 at 2, 27.2 at 3; 28.0 now at 2).  A unit
 // that lies in one CTA is written at once; of one that shares' borders cut, each CTA leaves its
 // (max, sum, unnormalised o) in the workspace, and the last of every 16 neighbours to do so adds
 // theirs, in CTA order whoever is last, until one is left: no CTA waits, no second launch.  A fence, an
@@ -268,9 +269,10 @@ __global__ void __launch_bounds__(256, 6) append_kernel(const AppendArgs a) {
 // scaled for that by a power of two per head to fp16's upper range: components of q down to 2^-30 of the
 // head's largest are exact, the others off by 2^-38 of it at most.
 //
-// Measured: 64 streams of 0 to 8k, 32/8 heads x 128, pages of 16, 183 us (5.9 TB/s, 90 % of a copy); 4 x 64k
-// in int8 101 us (5.5 TB/s; issue-bound next); 32 streams of 0 to 2k, 12 heads x 64, 27.5 us; one stream
-// of 4k, 4/1 x 256, 12.4 us, a chain of waits.
+// Measured back to back: 64 streams of 0 to 8k, 32/8 heads x 128, pages of 16, 182 us (5.9 TB/s, 90 % of a copy);
+// 4 x 64k in int8 117 us (4.7 TB/s; 137 us in calls of a second and more, under lower clocks), bound by its
+// instructions: 60 % of the issue slots with 3 warps a scheduler; 32 streams of 0 to 2k, 12 heads x 64, 28.0 us; one
+// stream of 4k, 4/1 x 256, 13.4 us, a chain of waits.
 constexpr int kWarps = 4, kStep = 16, kTileKeys = kWarps * kStep;
 
 struct AttnArgs {
@@ -311,7 +313,7 @@ struct AttnShape {
     static_assert(kPair == 1 || kJoin >= 2 * kWarps * kPair * 32 * NT * 16, "a pair's scores, twice, lie there too");
     static constexpr int kQRow = D + 8;
     static constexpr int kQ = kHeads * kQRow * 2 + kHeads * 4;           // q, and an int8 pool's factors
-    static constexpr bool kQInRegs = !(kPart == 256 && NT == 2);             // 64 registers of q beside 128 of o would spill
+    static constexpr bool kQInRegs = !(kPart == 256 && NT == 2);             // 64 registers of q beside 128 of o would not fit (without, int8 still spills 164 bytes)
     static constexpr int kSmem = kRing + kJoin + kQ;
     static_assert(kSmem + 2048 <= 227 * 1024, "shared memory");
     static constexpr int kCtas = 3 * (kSmem + 1800) <= 228 * 1024 ? 3 : 2 * (kSmem + 1800) <= 228 * 1024 ? 2 : 1;
@@ -469,12 +471,14 @@ __global__ void __launch_bounds__((AttnShape<D, I8, NT>::kThreads), (AttnShape<D
         empty_streams();
         return;
     }
-    // Short units, one CTA to each: its own steps take less than a join would (32 streams x 5 heads of 3
-    // tiles 7.5 us, in parts 9.8; 6 x 3 of up to 10 tiles 12.6 us, in parts 9.0).  Else no
+    // Short units, one CTA to each: its own steps take less than a join would (6 streams x 3 heads x 64 of 2
+    // tiles 5.8 us, in parts 7.7, of 4 tiles 7.0 and 7.8; 32 x 5 x 128 of 3 tiles 9.0 and 8.7; beyond, 6 x 3 of up
+    // to 10 tiles 12.6 us so, 8.4 in parts).  Else no
     // share is empty, so that a unit's parts lie in consecutive CTAs (one may hold an end alone): up to 64
-    // tiles a unit, no more CTAs than make 16 parts of the longest (one unit of 64 tiles: 13.2 us, in 8 parts
-    // 18.3, in 32 13.5); units of one length and few tiles, as many CTAs to each, whose parts then
-    // all have an end (64 units of 8 tiles: 14.3 us, else 19.0)
+    // tiles a unit, no more CTAs than make 16 parts of the longest (one unit of 32 tiles 10.9 us, else 12.3; of 64
+    // 13.4 and 12.5, 16 such units 13.9 and 16.3; past the border, 16 units of 65 tiles 16.4 us, within the rule 14.2,
+    // but one of 65 12.4 and 14.6, of 128 12.3 and 19.0); units of one length and few tiles, as many CTAs to each, whose
+    // parts then all have an end (64 units of 8 tiles 14.3 us, else 15.7; 160 of 8 15.1 and 18.5)
     const bool apart = live_units <= (Int)gridDim.x && longest <= S::kApartTiles;
     Int want = min((Int)gridDim.x, total);
     if (longest <= 4 * kJoinWays) want = min(want, total * kJoinWays / longest);
